@@ -25,7 +25,7 @@ struct DitLnParams {
   int ldx, ldy, C, rows, H, W; float eps; int mode;
 };
 template <class T>
-STAR_GLOBAL void dit_ln_kernel(const DitLnParams p) {
+STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256) dit_ln_kernel(const DitLnParams p) {
   constexpr int CPL = 8;     // 16-B chunks per lane: C <= 64 * 8 * 8 = 4096
   const int lane = threadIdx.x & 63;
   const int row = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
