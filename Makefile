@@ -21,6 +21,7 @@ emu: tools/hostemu/libstar_emu.so
 # masked scores are finite (-1e30 / -30000), so NaNs can only come from NaN inputs and propagate either way
 build/hip/attn.o: HIPFLAGS += -fno-honor-nans -fno-slp-vectorize
 build/hip/attn7.o: HIPFLAGS += -fno-honor-nans -fno-slp-vectorize -mllvm -amdgpu-mfma-vgpr-form
+build/hip/pattn.o build/bench/pattn.o: HIPFLAGS += -fno-slp-vectorize
 build/hip/gemm_as.o: HIPFLAGS += -fno-slp-vectorize -mllvm -amdgpu-mfma-vgpr-form
 build/hip/gemm_tq.o: HIPFLAGS += -fno-honor-nans -fno-slp-vectorize -mllvm -amdgpu-mfma-vgpr-form
 # precise header dependencies (-MMD): touching norm.h no longer recompiles the GEMM instantiation units (minutes each).

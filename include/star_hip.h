@@ -166,6 +166,66 @@ int star_layer_norm_rowab(star_ctx* ctx, const void* x, int32_t ldx, float* rowa
  * (star_gemm_rowstats): 16 x parts bytes are read per row instead of the row.  mode 3: maps[row] = (max, mean), rowab unused. */
 int star_layer_norm_rowab_from_partials(star_ctx* ctx, const float* ln_partial, int32_t parts, float* rowab, int32_t rows, int32_t C,
                                         float eps, int32_t mode, const float* gate_w, float* maps, int32_t H, int32_t W);
+/* nn.LayerNorm in training (what fine-tuning the norms of the blocks above needs, video_super_resolution/scripts/train_sr.py:648-731):
+ * the forward pass that keeps its row statistics, and the backward pass.  x, y, dy, dx: rows in the context's 16-bit type; gamma, beta and
+ * their gradients fp32 [C], null for a norm without them; any C up to 16384, any row strides >= C (multiples of 8 with 16-byte aligned
+ * pointers take the fast path).  y may be x, and dx may be x or dy.
+ *   stats[row] = (mean, 1 / sqrt(var + eps)), fp32 pairs (null: not kept)
+ *   dx = rstd (a - mean(a) - xh mean(a xh)), a = dy gamma;  dgamma = sum_rows dy xh;  dbeta = sum_rows dy  (either may be null)
+ * The row sums go through a workspace of star_layer_norm_bwd_workspace() bytes (none where both are null) that the caller owns and
+ * that the call overwrites: calls that may run at the same time, captured graphs among them, need one each.  No atomics: the same call
+ * gives the same bits.  rows = 0 writes zeros to dgamma and dbeta. */
+int star_layer_norm_train(star_ctx* ctx, const void* x, int64_t ldx, void* y, int64_t ldy, const float* gamma, const float* beta, float* stats,
+                          int32_t rows, int32_t C, float eps);
+size_t star_layer_norm_bwd_workspace(star_ctx* ctx, int32_t rows, int32_t C);
+int star_layer_norm_bwd(star_ctx* ctx, const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* stats, const float* gamma, void* dx,
+                        int64_t lddx, float* dgamma, float* dbeta, int32_t rows, int32_t C, void* workspace, size_t workspace_bytes);
+
+/* Attention whose scores depend on positions: a sliding window with first tokens that stay visible, lengths and query positions per sequence
+ * (padded batches, caches), grouped heads, and a learned relative position bias by buckets.  What star_attn_fwd does not do for long
+ * videos (text tokens first, then the frames: sinks = text tokens, window = some frames either way), for streaming against a cache of earlier
+ * frames, and for text encoders with a bucketed bias.  Head h uses columns [64 h, 64 h + 64) of Q, O and columns of head
+ * h / (heads / kv_heads) of K, V.
+ *   p = q_start[b] + i                                          (q_start null: Nk - Nq + i)
+ *   key j is visible to row i iff 0 <= j < kv_len[b] (null: Nk), j <= p + right, and (j >= p - left or j < sinks)
+ *   s_ij = scale q_i k_j + bias_table[bias_buckets[clamp(j - p, -R, R) + R]][h],  R = bias_range
+ *   O_i = sum_j softmax_j(s_ij) V_j over the visible keys;  lse_i = log sum_j exp s_ij;  a row that sees no key: O = 0, lse = -inf
+ * A token at a time is Nq = 1 against the cache (Nk its capacity, kv_len the keys in hand, q_start = kv_len - 1).  Values of kv_len outside
+ * [0, Nk] and buckets outside [0, num_buckets) are clamped to it, q_start to +-2^29.  K and V rows that no query row of a 128-row block
+ * (256 for long inputs) sees are not read; a NaN or an infinity in a V row (backward: also K, Q, dO rows) may reach the other rows of the
+ * block that the row belongs to.  Sums are fp32; probabilities (and dS) are rounded to the 16-bit type for the second product.
+ * The backward pass takes lse from the forward pass; gradients of heads, or of K and V, that are shared are sums over what shares them. */
+typedef struct star_pos_attn_desc {
+  const void* Q; const void* K; const void* V; void* O;
+  float* lse;                        /* fp32 [batch][heads][Nq]; forward: null if not wanted; backward: read */
+  int32_t ldq, ldk, ldv, ldo;        /* row strides in elements, multiples of 8 */
+  int64_t bsq, bsk, bsv, bso;        /* batch strides in elements, multiples of 8; bsk = bsv = 0: shared by all batches */
+  int32_t Nq, Nk, heads, kv_heads, batch;
+  float scale;
+  int32_t left, right;               /* window either way of the query's position; negative: no limit.  causal: right = 0 */
+  int32_t sinks;                     /* the first `sinks` keys are visible past the left end of the window too */
+  int32_t num_buckets, bias_range;   /* bias_range <= 1024 */
+  const int32_t* q_start; const int32_t* kv_len;              /* device int32 [batch] or null */
+  const float* bias_table;           /* device fp32 [num_buckets][heads] or null: no bias */
+  const int32_t* bias_buckets;       /* device int32 [2 * bias_range + 1] (star_rel_buckets), with the table */
+  void* workspace; size_t workspace_bytes;                    /* star_pos_attn_workspace() bytes, 16-byte aligned, overwritten: one for each call that may run at the same time */
+} star_pos_attn_desc;
+typedef struct star_pos_attn_grads {
+  const void* dO; void* dQ; void* dK; void* dV;               /* laid out like O, Q, K, V; shared K and V: dK and dV of one batch */
+  int32_t lddo, lddq, lddk, lddv;
+  int64_t bsdo, bsdq, bsdk, bsdv;
+  float* dbias_table;                /* fp32 [num_buckets][heads], with the table */
+} star_pos_attn_grads;
+size_t star_pos_attn_workspace(star_ctx* ctx, const star_pos_attn_desc* d, int32_t backward);
+int star_pos_attn_fwd(star_ctx* ctx, const star_pos_attn_desc* d);
+/* d as in the forward pass (O is not read); every element of dQ, dK, dV and dbias_table is written.  No atomics on floats in memory: the same
+ * call gives the same bits. */
+int star_pos_attn_bwd(star_ctx* ctx, const star_pos_attn_desc* d, const star_pos_attn_grads* g);
+/* The buckets of relative positions j - p = -max_distance .. max_distance (host int32 [2 * max_distance + 1]) in the scheme of text encoders
+ * with a bucketed bias: half of the buckets one for each near distance, the rest by equal ratios up to max_distance, the last for all beyond;
+ * bidirectional: one half of all buckets for keys after the query; else keys after the query fall into bucket 0.  The borders are
+ * compared in whole numbers.  Non-zero for num_buckets outside [1, 256] (bidirectional: even), or max_distance outside (num_buckets / 4 or / 2, 1024]. */
+int star_rel_buckets(int32_t num_buckets, int32_t max_distance, int32_t bidirectional, int32_t* buckets);
 /* replaces: torch.cat([x, skip + control], dim=1) (unet_v2v.py:1792) and residual adds */
 int star_concat_add(star_ctx* ctx, const void* a, const void* b, const void* c, void* out, int32_t rows, int32_t C1, int32_t C2);
 int star_add(star_ctx* ctx, const void* a, const void* b, void* out, int64_t n);

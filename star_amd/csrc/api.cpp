@@ -35,6 +35,23 @@ void rt_note_launch_error(const char* what) {
 // CONTEXT's device, not the caller's current one
 #define STAR_ENTER(h) do { if (!(h)) return 1; rt::set_device((h)->c.device); } while (0)
 
+// the same for the training and position entry points, which a program calls between its own work on several devices: the caller's
+// current device is put back on the way out
+namespace {
+struct DeviceScope {
+  int prev, dev;
+  explicit DeviceScope(int d) : prev(rt::get_device()), dev(d) { if (prev != dev) rt::set_device(dev); }
+  ~DeviceScope() { if (prev >= 0 && prev != dev) rt::set_device(prev); }
+};
+}
+// nothing of C++ passes a C entry point: an exception (out of host memory) is an error like others
+#define STAR_GUARDED(h, body)                                            \
+  do {                                                                   \
+    if (!(h)) return 1;                                                  \
+    try { DeviceScope star_scope_((h)->c.device); body }                 \
+    catch (...) { return 1; }                                            \
+  } while (0)
+
 static int finish(star_ctx* h, int rc) {
   if (rc) { g_launch_err.clear(); return rc; }
   if (!g_launch_err.empty()) {
@@ -99,8 +116,10 @@ const char* star_last_error(star_ctx* h) { return h ? h->c.err.c_str() : "null c
 int star_set_stream(star_ctx* h, void* s) {
   // the arena hands freed blocks out again immediately on the assumption that all work is ordered on ONE stream: when the
   // caller moves to another stream, everything enqueued on the old one is drained first (rare: once per torch stream context)
-  if (h->c.stream != (hipStream_t)s) {
-    rt::set_device(h->c.device);
+  // (nothing to drain where the arena never held a block.  A stream under capture cannot be waited for, nor may a capture wait for what ran
+  // before it: what is captured runs later, in the order in which its graph is launched.)
+  if (h->c.stream != (hipStream_t)s && h->c.pool.total() != 0 && !rt::stream_capturing((hipStream_t)s) && !rt::stream_capturing(h->c.stream)) {
+    DeviceScope scope(h->c.device);
     if (rt::stream_sync(h->c.stream)) return h->c.fail(std::string("set_stream: sync of the previous stream failed: ") + rt::last_error_string());
   }
   h->c.stream = (hipStream_t)s;
@@ -217,6 +236,52 @@ int star_layer_norm_rowab(star_ctx* h, const void* x, int32_t ldx, float* rowab,
   if (!rowab) return finish(h, h->c.fail("layer_norm_rowab: null output"));
   if (mode == LN_STATS_ONLY) return finish(h, h->c.fail("layer_norm_rowab: mode 3 (maps only) has no row statistics; use star_layer_norm"));
   return finish(h, op_layer_norm(&h->c, x, ldx, nullptr, 8, nullptr, nullptr, rows, C, eps, mode, gate_w, maps, H, W, rowab));
+}
+int star_layer_norm_train(star_ctx* h, const void* x, int64_t ldx, void* y, int64_t ldy, const float* gamma, const float* beta, float* stats,
+                          int32_t rows, int32_t C, float eps) {
+  STAR_GUARDED(h, { return finish(h, op_layer_norm_train(&h->c, x, ldx, y, ldy, gamma, beta, stats, rows, C, eps)); });
+}
+size_t star_layer_norm_bwd_workspace(star_ctx* h, int32_t rows, int32_t C) { return h ? ln_train_bwd_workspace(&h->c, rows, C) : 0; }
+int star_layer_norm_bwd(star_ctx* h, const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* stats, const float* gamma, void* dx,
+                        int64_t lddx, float* dgamma, float* dbeta, int32_t rows, int32_t C, void* workspace, size_t workspace_bytes) {
+  STAR_GUARDED(h, {
+    return finish(h, op_layer_norm_bwd(&h->c, dy, lddy, x, ldx, stats, gamma, dx, lddx, dgamma, dbeta, rows, C, workspace, workspace_bytes));
+  });
+}
+static PAttnArgs pos_attn_args(const star_pos_attn_desc* d) {
+  PAttnArgs a;
+  a.Q = d->Q; a.K = d->K; a.V = d->V; a.O = d->O; a.lse = d->lse;
+  a.ldq = d->ldq; a.ldk = d->ldk; a.ldv = d->ldv; a.ldo = d->ldo;
+  a.bsq = d->bsq; a.bsk = d->bsk; a.bsv = d->bsv; a.bso = d->bso;
+  a.Nq = d->Nq; a.Nk = d->Nk; a.heads = d->heads; a.kv_heads = d->kv_heads; a.batch = d->batch;
+  a.scale = d->scale; a.left = d->left; a.right = d->right; a.sinks = d->sinks;
+  a.q_start = d->q_start; a.kv_len = d->kv_len;
+  a.table = d->bias_table; a.buckets = d->bias_buckets; a.num_buckets = d->num_buckets; a.R = d->bias_range;
+  a.workspace = d->workspace; a.workspace_bytes = d->workspace_bytes;
+  return a;
+}
+size_t star_pos_attn_workspace(star_ctx* h, const star_pos_attn_desc* d, int32_t backward) {
+  return h && d ? pos_attn_workspace(&h->c, pos_attn_args(d), backward != 0) : 0;
+}
+int star_pos_attn_fwd(star_ctx* h, const star_pos_attn_desc* d) {
+  STAR_GUARDED(h, {
+    if (!d) return finish(h, h->c.fail("pos_attn_fwd: null descriptor"));
+    return finish(h, op_pos_attn_fwd(&h->c, pos_attn_args(d)));
+  });
+}
+int star_pos_attn_bwd(star_ctx* h, const star_pos_attn_desc* d, const star_pos_attn_grads* g) {
+  STAR_GUARDED(h, {
+    if (!d || !g) return finish(h, h->c.fail("pos_attn_bwd: null descriptor"));
+    PAttnArgs a = pos_attn_args(d);
+    a.ldo = a.heads * 64; a.bso = 0;                     // O is not read
+    a.dO = g->dO; a.dQ = g->dQ; a.dK = g->dK; a.dV = g->dV;
+    a.lddo = g->lddo; a.lddq = g->lddq; a.lddk = g->lddk; a.lddv = g->lddv;
+    a.bsdo = g->bsdo; a.bsdq = g->bsdq; a.bsdk = g->bsdk; a.bsdv = g->bsdv;
+    return finish(h, op_pos_attn_bwd(&h->c, a, g->dbias_table));
+  });
+}
+int star_rel_buckets(int32_t num_buckets, int32_t max_distance, int32_t bidirectional, int32_t* buckets) {
+  try { return rel_buckets(num_buckets, max_distance, bidirectional != 0, buckets); } catch (...) { return 1; }
 }
 int star_concat_add(star_ctx* h, const void* a, const void* b, const void* c, void* out, int32_t rows, int32_t C1, int32_t C2) {
   STAR_ENTER(h);

@@ -107,6 +107,32 @@ int op_layer_norm(Ctx* ctx, const void* x, int ldx, void* y, int ldy, const floa
 // op_layer_norm with rowab / STATS_ONLY outputs, 16 x parts bytes read per row
 int op_layer_norm_from_partials(Ctx* ctx, const float* partial, int parts, int rows, int C, float eps, int mode, const float* gate_w,
                                 float* maps, int H, int W, float* rowab);
+// ln_train.cpp: LayerNorm that keeps its row statistics (stats[row] = (mean, rstd)), and its backward pass with the weight's gradient
+int op_layer_norm_train(Ctx* ctx, const void* x, long long ldx, void* y, long long ldy, const float* gamma, const float* beta, float* stats,
+                        int rows, int C, float eps);
+size_t ln_train_bwd_workspace(Ctx* ctx, int rows, int C);
+int op_layer_norm_bwd(Ctx* ctx, const void* dy, long long lddy, const void* x, long long ldx, const float* stats, const float* gamma, void* dx,
+                      long long lddx, float* dgamma, float* dbeta, int rows, int C, void* workspace, size_t workspace_bytes);
+
+// pattn.cpp: attention with a sliding window, first tokens that stay visible, lengths and positions per sequence, grouped heads and a
+// learned relative position bias by buckets (pattn.h); forward and backward
+struct PAttnArgs {
+  const void* Q = nullptr; const void* K = nullptr; const void* V = nullptr; void* O = nullptr; float* lse = nullptr;
+  const void* dO = nullptr; void* dQ = nullptr; void* dK = nullptr; void* dV = nullptr;
+  int ldq = 0, ldk = 0, ldv = 0, ldo = 0, lddo = 0, lddq = 0, lddk = 0, lddv = 0;
+  long long bsq = 0, bsk = 0, bsv = 0, bso = 0, bsdo = 0, bsdq = 0, bsdk = 0, bsdv = 0;
+  int Nq = 0, Nk = 0, heads = 0, kv_heads = 0, batch = 0;
+  float scale = 0.125f;
+  int left = -1, right = -1, sinks = 0;             // negative: no limit on that side
+  const int* q_start = nullptr; const int* kv_len = nullptr;
+  const float* table = nullptr; const int* buckets = nullptr; int num_buckets = 0, R = 0;
+  void* workspace = nullptr; size_t workspace_bytes = 0;
+};
+size_t pos_attn_workspace(Ctx* ctx, const PAttnArgs& a, bool backward);
+int op_pos_attn_fwd(Ctx* ctx, const PAttnArgs& a);
+int op_pos_attn_bwd(Ctx* ctx, const PAttnArgs& a, float* dtable);
+int rel_buckets(int num_buckets, int distance, bool bidirectional, int* out);
+
 int op_concat_add(Ctx* ctx, const void* a, const void* b, const void* c, void* out, int rows, int C1, int C2, float* gn_partial = nullptr);
 int op_add(Ctx* ctx, const void* a, const void* b, void* out, long long n);
 int op_stem_im2col(Ctx* ctx, const float* latent, void* out, int Cl, int F, int H, int W, bool frame_major = false);

@@ -1,0 +1,442 @@
+// pattn.h -- attention whose scores depend on positions: a sliding window with first tokens that stay visible, key lengths per sequence,
+// query positions in a cache, and a learned relative position bias by buckets; head dim 64, grouped heads.  Forward; the backward pass
+// is in pattn_bwd.h.
+//
+//   p_i = q_start[b] + i;  key j is visible to row i for 0 <= j < kv_len[b], j <= p + right, and (j >= p - left or j < sinks)
+//   s_ij = scale q_i k_j + table[buckets[clamp(j - p, -R, R) + R]][h];  O = softmax over the visible keys of s, times V; a row that sees
+//   no key: O = 0, lse = -inf.  lse_i = log sum_j exp s_ij.
+//
+// Layout as in attn5.h: S^T = K Q^T with the operands swapped, so that a lane owns one query row and its probabilities are the B operand
+// of O^T = V^T P^T in place; K / V tiles of 64 keys in LDS by DMA, two buffers.  What differs, and why:
+//   * Q is not scaled before the product (that would round it to 16 bits once more; with the rounding of P the outputs would be off by more
+//     than 1.5 x their own rounding): the scale, the bias and the running maximum meet in one fma per score.
+//   * A tile is "plain" when every row of the workgroup sees all of its keys and the bias is one constant there (past +-R it is: the far
+//     tiles, nearly all of a long sequence).  Plain tiles take the lazy path: P = exp2(fma(s, c, off)) against the running maximum as it
+//     stands, the row sum as overflow probe.  Every other tile, and every tile until each row of the wave has seen one, takes the
+//     exact path: masks and bias per score, the tile's maximum, rescale.  Tiles that no row of the workgroup sees are not visited.
+//   * Rows of the heads that share a K / V head are packed token-major into one workgroup's rows (GP of them), so that a group reads its
+//     keys once; with a bias a workgroup keeps to one head (one table column in LDS).
+//   * K / V rows that no row of the workgroup sees are staged as zeros through the descriptor's range check: what lies behind kv_len or
+//     outside the window is not read.
+//   * Few rows against long key ranges (a decoding step): the key tiles are dealt to NSPLIT workgroups, each writes its (m, l, O) of the
+//     rows in fp32, pattn_combine_kernel joins them in a fixed order.
+// NQ: 32-row blocks per wave (2: 256-row workgroups for long inputs, 1: 128 rows, more workgroups); NW = 1: a wave by itself, 32 rows.
+// COMP: P is rounded to the 16-bit type, and so is what the rounding left, and both take part in the second product: O is then off by its own
+// rounding alone.  Four more matrix instructions per 32 x 32 block, taken where they do not show: short rows (a few dozen roundings do not
+// average out there either) and the single-wave form, which waits for its keys.
+#pragma once
+#include "attn.h"
+
+namespace star {
+
+struct PAttnParams {
+  const void* Q; const void* K; const void* V; void* O; float* lse;
+  const void* dO; void* dQ; void* dK; void* dV;
+  int ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;      // row strides (elements)
+  long long bsq, bsk, bsv, bso, bsdo, bsdq, bsdk, bsdv; // batch strides (elements)
+  int Nq, Nk, heads, kv_heads, batch;
+  int gp;                             // heads packed into one unit's rows (1, or heads / kv_heads)
+  int rows;                           // gp * Nq
+  float c, scale;                     // scale * log2(e), scale
+  int left, right, sinks;             // left / right past every position: no limit
+  const int* q_start; const int* kv_len;
+  int start0;                         // position of row 0 where q_start is null
+  const float* table; const int* buckets; int num_buckets, R;
+  int nblk, nsplit;                   // row blocks per unit; key splits
+  long long items;                    // units * nblk * nsplit
+  int swz;                            // 1: each XCD walks a contiguous run of items
+  float* part;                        // nsplit > 1: [unit][split][rows][68]: O[64], m, l
+  // backward
+  float* st_lse; float* st_delta; float* st_amax;      // [unit][rows]
+  float* dsum;                        // [item][2R + 1] sums of dS by relative position
+  int sblk, split_s, split_n;         // dK / dV: the first sblk key blocks (those of the first tokens) in split_s parts each, the others in split_n
+};
+
+constexpr int PA_KT = 64, PA_TILE = PA_KT * 128;       // keys per tile, bytes of a K or V tile
+constexpr int PA_PART = 68;                            // floats per row of a split's partial result (16-byte rows)
+constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
+constexpr float PA_NINF = -__builtin_inff();
+
+struct PRange { int n, qs; };                          // keys in hand, position of row 0 -- both clamped to what the kernels can index
+STAR_DEV PRange pa_range(const PAttnParams& p, int b) {
+  int n = p.kv_len ? p.kv_len[b] : p.Nk;
+  n = n < 0 ? 0 : n > p.Nk ? p.Nk : n;
+  int s = p.q_start ? p.q_start[b] : p.start0;
+  const int lim = 1 << 29;
+  s = s < -lim ? -lim : s > lim ? lim : s;
+  return PRange{wave_uniform(n), wave_uniform(s)};
+}
+// the window [lo, hi) of the row at position pos, and the count of first tokens beside it
+STAR_DEV int pa_hi(const PAttnParams& p, int n, int pos) { const int h = pos + p.right + 1; return h < 0 ? 0 : h > n ? n : h; }
+STAR_DEV int pa_lo(const PAttnParams& p, int pos) { const int l = pos - p.left; return l < 0 ? 0 : l; }
+
+// the key tiles that rows at positions [p0, p1] see: [0, na) and [b0, b0 + nb)
+struct PTiles { int na, b0, nb, lo, hi, sk; };
+STAR_DEV PTiles pa_tiles(const PAttnParams& p, int n, int p0, int p1) {
+  PTiles t;
+  t.hi = pa_hi(p, n, p1);
+  t.lo = pa_lo(p, p0);
+  if (t.lo > t.hi) t.lo = t.hi;
+  t.sk = p.sinks < t.hi ? p.sinks : t.hi;
+  t.na = (t.sk + PA_KT - 1) / PA_KT;
+  t.b0 = t.lo / PA_KT;
+  const int end = (t.hi + PA_KT - 1) / PA_KT;
+  if (t.b0 < t.na) t.b0 = t.na;
+  t.nb = t.lo < t.hi && end > t.b0 ? end - t.b0 : 0;
+  return t;
+}
+
+// which item this workgroup has; units (batch, head group) outermost, then row blocks, then splits
+STAR_DEV long long pa_item(const PAttnParams& p) {
+  const long long bid = blockIdx.x;
+  if (!p.swz) return bid;
+  const long long per = (p.items + 7) / 8, slot = bid >> 3;
+  return slot >= per ? p.items : (bid & 7) * per + slot;
+}
+
+// the bias of one head by relative position, times log2(e), in LDS: tab[i] belongs to j - p = i - R.  The type's lowest value stays finite
+template <int NT>
+STAR_DEV void pa_bias_table(const PAttnParams& p, int head, float* tab) {
+  for (int i = threadIdx.x; i < 2 * p.R + 1; i += NT) {
+    int k = p.buckets[i];
+    k = k < 0 ? 0 : k >= p.num_buckets ? p.num_buckets - 1 : k;
+    const float v = p.table[(size_t)k * p.heads + head];
+    float w = v * PA_LOG2E;
+    if (w == PA_NINF && v != PA_NINF) w = -3.4028235e38f;
+    tab[i] = w;
+  }
+}
+
+// copies rows of 64 elements (128 bytes) into a swizzled LDS tile, 16 bytes per lane and step; rows that `ok` refuses become zeros.
+// base: wave-uniform address of the tile's first row; the byte offset of a row from it stays below 2^31 (the launcher checks strides)
+template <int NT, class OFF>
+STAR_DEV void pa_stage(const void* base, char* smem, int dst, int tid, int wv, OFF off) {
+  const BufDesc d = make_desc(base, GLDS_BUF_RANGE);
+#pragma unroll
+  for (int j = 0; j < 512 / NT; ++j) {
+    const int r = (j * NT + tid) >> 3;
+    const int ch = (tid & 7) ^ ((r >> 1) & 7);
+    glds16_desc(d, off(r, ch), 0, smem + wave_uniform(dst + (j * NT + wv * 64) * 16));
+  }
+}
+
+// row of a unit -> token and head within the unit
+// (a division's result is in vector registers even where it is the same for all lanes: what steers the DMA goes through wave_uniform)
+struct PRow { int i, g; };
+STAR_DEV PRow pa_row(const PAttnParams& p, int r) {
+  if (p.gp == 1) return PRow{r, 0};
+  const int i = r / p.gp;
+  return PRow{i, r - i * p.gp};
+}
+
+// eight rows of d per lane half: acc[db] holds d = 32 db + (r & 3) + 8 (r >> 2) + 4 h2 of the lane's row; 16-byte stores
+template <class T>
+STAR_DEV void pa_store_row(const f32x16* acc, float mul, T* row, bool ok) {
+  const int h2 = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int db = 0; db < 2; ++db)
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      u32x2 w[2];
+#pragma unroll
+      for (int gg = 0; gg < 2; ++gg) {
+        vec<T, 4> o4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o4[e] = from_f32<T>(acc[db][(2 * a + gg) * 4 + e] * mul);
+        w[gg] = __builtin_bit_cast(u32x2, o4);
+      }
+      const u32x2 x0 = permlane32_swap(w[0][0], w[1][0]);
+      const u32x2 x1 = permlane32_swap(w[0][1], w[1][1]);
+      u32x4 out;
+      out[0] = x0[0]; out[1] = x1[0]; out[2] = x0[1]; out[3] = x1[1];
+      if (ok) *reinterpret_cast<u32x4*>(row + 32 * db + 16 * a + 8 * h2) = out;
+    }
+}
+
+template <class T, int BIAS, int NQ, int NW, int COMP>
+STAR_GLOBAL void STAR_LAUNCH_BOUNDS(NW * 64, NW == 1 ? 1 : 2)
+pattn_fwd_kernel(const PAttnParams p) {
+  constexpr int NT = NW * 64, QW = 32 * NQ, QB = NW * QW;
+  constexpr float LAZY_BIG = 1024.0f;
+  char* smem = dyn_smem();                             // two buffers of (K tile | V tile), then the bias table
+  float* tab = reinterpret_cast<float*>(smem + 4 * PA_TILE);
+  const long long item = pa_item(p);
+  if (item >= p.items) return;
+  const int tid = threadIdx.x, lane = tid & 63, wv = wave_uniform(tid >> 6);
+  const int h2 = lane >> 5, lq = lane & 31;
+  const int split = wave_uniform((int)(item % p.nsplit));
+  const long long ub = item / p.nsplit;
+  const int qb = wave_uniform(p.nblk - 1 - (int)(ub % p.nblk));      // the rows that see most keys first
+  const int unit = wave_uniform((int)(ub / p.nblk));
+  const int upb = p.heads / p.gp;                      // units per sequence
+  const int b = wave_uniform(unit / upb), head0 = wave_uniform((unit - b * upb) * p.gp);
+  const int kvh = wave_uniform(head0 / (p.heads / p.kv_heads));
+  const PRange rg = pa_range(p, b);
+  const int n = rg.n;
+  const T* Qg = (const T*)p.Q + (size_t)b * p.bsq + head0 * 64;
+  const T* Kg = (const T*)p.K + (size_t)b * p.bsk + kvh * 64;
+  const T* Vg = (const T*)p.V + (size_t)b * p.bsv + kvh * 64;
+
+  const int r_base = qb * QB;
+  const int r_last = r_base + QB - 1 < p.rows - 1 ? r_base + QB - 1 : p.rows - 1;
+  const int p0 = wave_uniform(rg.qs + pa_row(p, r_base).i), p1 = wave_uniform(rg.qs + pa_row(p, r_last).i);
+  const PTiles tl = pa_tiles(p, n, p0, p1);
+  // a tile is seen whole by every row if it ends before hi_min and begins at lo_max or lies among the first tokens
+  const int hi_min = pa_hi(p, n, p0), lo_max = pa_lo(p, p1);
+
+  vec<T, 8> qf[NQ][4];
+  int pos[NQ];                                         // position of the lane's row
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+    int r = r_base + wv * QW + qi * 32 + lq;
+    if (r > p.rows - 1) r = p.rows - 1;
+    const PRow rw = pa_row(p, r);
+    pos[qi] = rg.qs + rw.i;
+    const T* q = Qg + (size_t)rw.i * p.ldq + rw.g * 64;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) qf[qi][ks] = *reinterpret_cast<const vec<T, 8>*>(q + ks * 16 + h2 * 8);
+  }
+  float far_l = 0.f, far_r = 0.f;
+  if constexpr (BIAS) {
+    pa_bias_table<NT>(p, head0, tab);
+    block_sync();
+    far_l = tab[0]; far_r = tab[2 * p.R];
+  }
+
+  const int total = tl.na + tl.nb;
+  const int per = wave_uniform((total + p.nsplit - 1) / p.nsplit);
+  const int it0 = split * per < total ? split * per : total, it1 = it0 + per < total ? it0 + per : total;
+  auto tile_of = [&](int it) STAR_ALWAYS_INLINE { return it < tl.na ? it : it - tl.na + tl.b0; };
+  auto stage = [&](int it, int buf) STAR_ALWAYS_INLINE {
+    const int t = tile_of(it), k0 = t * PA_KT;
+    const int kd = buf * 2 * PA_TILE;
+    const T* kb = Kg + (size_t)k0 * p.ldk;
+    const T* vb = Vg + (size_t)k0 * p.ldv;
+    const bool whole = k0 + PA_KT <= tl.hi && (k0 >= tl.lo || k0 + PA_KT <= tl.sk);
+    if (whole) {
+      pa_stage<NT>(kb, smem, kd, tid, wv, [&](int r, int ch) { return (uint32_t)(r * p.ldk + ch * 8) * 2u; });
+      pa_stage<NT>(vb, smem, kd + PA_TILE, tid, wv, [&](int r, int ch) { return (uint32_t)(r * p.ldv + ch * 8) * 2u; });
+    } else {
+      auto seen = [&](int r) { const int key = k0 + r; return key < tl.hi && (key >= tl.lo || key < tl.sk); };
+      pa_stage<NT>(kb, smem, kd, tid, wv, [&](int r, int ch) { return seen(r) ? (uint32_t)(r * p.ldk + ch * 8) * 2u : GLDS_BUF_OOB; });
+      pa_stage<NT>(vb, smem, kd + PA_TILE, tid, wv, [&](int r, int ch) { return seen(r) ? (uint32_t)(r * p.ldv + ch * 8) * 2u : GLDS_BUF_OOB; });
+    }
+  };
+
+  // loop-invariant fragment addresses (attn5.h): K row kb * 32 + lq, chunk ks * 2 + h2; V^T by transposing reads
+  const char* kfo[4];
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) kfo[ks] = opaque(smem + swz_off(lq, ks * 2 + h2));
+  const char* vfo[2][2];
+  {
+    const int i = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int db = 0; db < 2; ++db) {
+        const int key = 8 * half + 4 * h2 + (i >> 2), d = 32 * db + 16 * (g & 1) + 4 * (i & 3);
+        vfo[half][db] = opaque(smem + PA_TILE + swz_off(key, d >> 3) + (d & 7) * 2);
+      }
+  }
+
+  f32x16 oacc[NQ][2];
+#pragma unroll
+  for (int a = 0; a < NQ; ++a)
+#pragma unroll
+    for (int c2 = 0; c2 < 2; ++c2)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) oacc[a][c2][r] = 0.f;
+  float m_run[NQ], l_run[NQ];                          // base 2; m = -inf: the row has seen no key yet
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) { m_run[qi] = PA_NINF; l_run[qi] = 0.f; }
+  bool fresh = true;                                   // wave-uniform: some row may not have seen a key yet
+
+  auto tile = [&](int it, int buf) STAR_ALWAYS_INLINE {
+    const int k0 = tile_of(it) * PA_KT;
+    const int bofs = buf * 2 * PA_TILE;
+    const bool masked = !(k0 + PA_KT <= hi_min && (k0 >= lo_max || k0 + PA_KT <= p.sinks));
+    bool near = false;
+    float far = 0.f;
+    if constexpr (BIAS) {
+      const bool fl = k0 + PA_KT - 1 - p0 <= -p.R, fr = k0 - p1 >= p.R;
+      near = !(fl || fr);
+      far = fl ? far_l : far_r;
+    }
+    f32x16 s[NQ][2];
+    auto scores = [&]() STAR_ALWAYS_INLINE {
+#pragma unroll
+      for (int a = 0; a < NQ; ++a)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[a][kb][r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const vec<T, 8> kf = *reinterpret_cast<const vec<T, 8>*>(kfo[ks] + bofs + kb * 4096);
+#pragma unroll
+          for (int qi = 0; qi < NQ; ++qi) s[qi][kb] = mfma32<T>(kf, qf[qi][ks], s[qi][kb]);
+        }
+    };
+    vec<T, 8> pf[NQ][4], pl[COMP ? NQ : 1][4];
+    float lsum[NQ];
+    // P = exp2(fma(s, c, off)): the row sum in four chains of fp32 adds on the unrounded values
+    auto expo = [&](int qi, float c, float off) STAR_ALWAYS_INLINE {
+      float ls0 = 0.f, ls1 = 0.f, ls2 = 0.f, ls3 = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          vec<T, 8> pk, pr;
+#pragma unroll
+          for (int e = 0; e < 8; e += 4) {
+            const float a0 = fast_exp2(__builtin_fmaf(s[qi][kb][8 * u + e], c, off)), a1 = fast_exp2(__builtin_fmaf(s[qi][kb][8 * u + e + 1], c, off));
+            const float a2 = fast_exp2(__builtin_fmaf(s[qi][kb][8 * u + e + 2], c, off)), a3 = fast_exp2(__builtin_fmaf(s[qi][kb][8 * u + e + 3], c, off));
+            ls0 += a0; ls1 += a1; ls2 += a2; ls3 += a3;
+            pk[e] = from_f32<T>(a0); pk[e + 1] = from_f32<T>(a1); pk[e + 2] = from_f32<T>(a2); pk[e + 3] = from_f32<T>(a3);
+            if constexpr (COMP) {
+              pr[e] = from_f32<T>(a0 - to_f32<T>(pk[e])); pr[e + 1] = from_f32<T>(a1 - to_f32<T>(pk[e + 1]));
+              pr[e + 2] = from_f32<T>(a2 - to_f32<T>(pk[e + 2])); pr[e + 3] = from_f32<T>(a3 - to_f32<T>(pk[e + 3]));
+            }
+          }
+          pf[qi][kb * 2 + u] = pk;
+          if constexpr (COMP) pl[qi][kb * 2 + u] = pr;
+        }
+      lsum[qi] = (ls0 + ls1) + (ls2 + ls3);
+    };
+    bool exact = masked || near || fresh;
+    if (!exact) {
+      scores();
+      bool bad = false;
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi) {
+        expo(qi, p.c, far - m_run[qi]);
+        bad = bad || !(lsum[qi] <= LAZY_BIG);
+      }
+      exact = wave_any(bad);                           // some P is large (or overflowed): move the maximum and do the tile again
+    }
+    if (exact) {
+      scores();                                        // (the K tile is still there; scores kept beside P would not fit the registers)
+      bool unseen = false;
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi) {
+        const int hi = pa_hi(p, n, pos[qi]), lo = pa_lo(p, pos[qi]);
+        float mx = PA_NINF;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = k0 + kb * 32 + (r & 3) + 8 * (r >> 2) + 4 * h2;
+            float bias = far;
+            if constexpr (BIAS) {
+              if (near) {
+                int i = key - pos[qi];
+                i = i < -p.R ? -p.R : i > p.R ? p.R : i;
+                bias = tab[i + p.R];
+              }
+            }
+            float y = __builtin_fmaf(s[qi][kb][r], p.c, bias);
+            if (masked && !(key < hi && (key >= lo || key < p.sinks))) y = PA_NINF;
+            s[qi][kb][r] = y;
+            mx = fmaxf(mx, y);
+          }
+        mx = pair_max(mx);
+        const float m_new = fmaxf(m_run[qi], mx);
+        const float alpha = m_new == PA_NINF ? 1.f : fast_exp2(m_run[qi] - m_new);
+        m_run[qi] = m_new;
+        l_run[qi] *= alpha;
+#pragma unroll
+        for (int db = 0; db < 2; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) oacc[qi][db][r] *= alpha;
+        unseen = unseen || m_new == PA_NINF;
+        expo(qi, 1.f, m_new == PA_NINF ? 0.f : -m_new);
+      }
+      fresh = wave_any(unseen);
+    }
+#pragma unroll
+    for (int qi = 0; qi < NQ; ++qi) l_run[qi] += lsum[qi];
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int db = 0; db < 2; ++db) {
+        vec<T, 8> vf;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const vec<T, 4> r = lds_read_tr<T>(vfo[half][db] + bofs + tt * 2048);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vf[half * 4 + e] = r[e];
+        }
+#pragma unroll
+        for (int qi = 0; qi < NQ; ++qi) {
+          oacc[qi][db] = mfma32<T>(vf, pf[qi][tt], oacc[qi][db]);
+          if constexpr (COMP) oacc[qi][db] = mfma32<T>(vf, pl[qi][tt], oacc[qi][db]);
+        }
+      }
+  };
+
+  glds_wait();                                         // the Q loads are done before the first hand-written LDS-DMA
+  if (it0 < it1) stage(it0, 0);
+  for (int it = it0; it < it1; ++it) {
+    const int buf = wave_uniform((it - it0) & 1);
+    glds_wait(); block_sync();
+    if (it + 1 < it1) stage(it + 1, buf ^ 1);
+    tile(it, buf);
+  }
+
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+    const float l = pair_sum(l_run[qi]);
+    const int r = r_base + wv * QW + qi * 32 + lq;
+    const bool ok = r < p.rows;
+    const PRow rw = pa_row(p, ok ? r : p.rows - 1);
+    if (p.nsplit > 1) {
+      if (ok) {
+        float* o = p.part + (((size_t)unit * p.nsplit + split) * p.rows + r) * PA_PART;
+#pragma unroll
+        for (int db = 0; db < 2; ++db)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = oacc[qi][db][g * 4 + e];
+            *reinterpret_cast<f32x4*>(o + 32 * db + 8 * g + 4 * h2) = v;
+          }
+        if (h2 == 0) { o[64] = m_run[qi]; o[65] = l; }
+      }
+    } else {
+      pa_store_row<T>(oacc[qi], l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l, (T*)p.O + (size_t)b * p.bso + (size_t)rw.i * p.ldo + (head0 + rw.g) * 64, ok);
+      if (p.lse && ok && h2 == 0)
+        p.lse[((size_t)b * p.heads + head0 + rw.g) * p.Nq + rw.i] = l == 0.f ? PA_NINF : (m_run[qi] + __builtin_log2f(l)) * PA_LN2;
+    }
+  }
+}
+
+// joins the splits of a row, in their order: one wave per row, lane = d
+template <class T>
+STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256)
+pattn_combine_kernel(const PAttnParams p) {
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int upb = p.heads / p.gp;
+  if (row >= (long long)p.batch * upb * p.rows) return;
+  const int unit = (int)(row / p.rows), r = (int)(row - (long long)unit * p.rows);
+  const float* base = p.part + ((size_t)unit * p.nsplit * p.rows + r) * PA_PART;
+  const size_t step = (size_t)p.rows * PA_PART;
+  float m = PA_NINF;
+  for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, base[s * step + 64]);
+  float l = 0.f, o = 0.f;
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float ms = base[s * step + 64];
+    const float w = ms == PA_NINF ? 0.f : fast_exp2(ms - m);
+    l += w * base[s * step + 65];
+    o += w * base[s * step + lane];
+  }
+  const PRow rw = pa_row(p, r);
+  const int b = unit / upb, head = (unit - b * upb) * p.gp + rw.g;
+  ((T*)p.O)[(size_t)b * p.bso + (size_t)rw.i * p.ldo + head * 64 + lane] = from_f32<T>(l > 0.f ? o / l : l == 0.f ? 0.f : l);
+  if (p.lse && lane == 0) p.lse[((size_t)b * p.heads + head) * p.Nq + rw.i] = l == 0.f ? PA_NINF : (m + __builtin_log2f(l)) * PA_LN2;
+}
+
+}  // namespace star

@@ -1,0 +1,687 @@
+// pattn_bwd.h -- backward pass of the position-dependent attention (pattn.h).
+//
+//   P = exp(s - lse), dV = P^T dO, dP = dO V^T, delta = sum_j P dP, dS = P (dP - delta),
+//   dQ = scale dS K, dK = scale dS^T Q, dtable[k][h] = sum over the pairs of bucket k of dS
+//
+// Two kernels, so that every sum has one owner and a fixed order (no atomics): the same call gives the same bits.
+//   pattn_dq_kernel    a wave owns query rows and walks the keys twice.  First walk: delta, and the log-sum-exp once more (the caller's is
+//                      rounded to fp32 and in base e).  Second walk: dS, dQ, and the sums of dS by relative position.
+//   pattn_dkdv_kernel  a wave owns 32 keys and walks the query rows of every head of the group (and of every sequence, where the batch
+//                      shares K and V): dK, dV.
+// delta is not taken as rowsum(dO O): O is rounded to 16 bits and comes from rounded P, and where a softmax is peaked dP - delta is a small
+// difference -- the error of dQ and dK would be several times their own rounding.  The first walk costs 8 of 36 matrix instructions
+// per 32 x 32 block.  dP is the same sum in the same order in both kernels, so that a row with one visible key has dS = 0 exactly.
+// f16 only: P and dS are scaled by powers of two before they are rounded, so that long rows and small gradients do not fall
+// below f16's normal range: P by 2^10 (P <= 1), dS by the largest |dO| of the row (dQ) or of the rows walked so far (dK).
+// COMP: as in the forward pass, dS and P with what their rounding left, for short rows.
+// Key blocks that many rows see (those of the first tokens: every row), or few blocks on many compute units, are dealt to several
+// workgroups along the rows; each writes its part in fp32, pattn_dkdv_join_kernel adds the parts in their order.
+// Per 32 x 32 block and wave both kernels read 12 - 16 KB of LDS against 12 - 16 matrix instructions of 32 cycles: LDS bandwidth and the
+// vector work on the scores (about 36 cycles a score) are what bounds them.
+#pragma once
+#include "pattn.h"
+
+namespace star {
+
+// 2^e with |x| 2^e in [8, 16): the exponent as an integer, 0 for zero and non-finite x; within [-24, 40]
+STAR_DEV int pa_fit_exp(float x) {
+  const uint32_t ex = (__builtin_bit_cast(uint32_t, x) >> 23) & 255u;
+  if (ex == 0u) return x == 0.f ? 0 : 40;
+  if (ex == 255u) return 0;
+  const int e = 130 - (int)ex;
+  return e < -24 ? -24 : e > 40 ? 40 : e;
+}
+STAR_DEV float pa_pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
+
+template <class T>
+STAR_DEV float pa_absmax(const vec<T, 8>* f) {
+  float m = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, __builtin_fabsf(to_f32<T>(f[ks][e])));
+  return m;
+}
+
+// LDS add of this wave's own array: lanes of one call hit different words, and a wave's LDS operations run in order
+STAR_DEV void lds_add(float* p, float v) {
+#ifdef STAR_HOSTEMU
+  *p += v;
+#else
+  (void)__hip_atomic_fetch_add((__attribute__((address_space(3))) float*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+#endif
+}
+
+// the rounded value, and what that left
+template <class T, int COMP>
+STAR_DEV void pa_round(float v, T& hi, T& lo) {
+  hi = from_f32<T>(v);
+  if constexpr (COMP) lo = from_f32<T>(v - to_f32<T>(hi));
+}
+
+template <class T, int BIAS, int NQ, int COMP>
+STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256, 2)
+pattn_dq_kernel(const PAttnParams p) {
+  constexpr int NT = 256, QW = 32 * NQ, QB = 4 * QW;
+  char* smem = dyn_smem();                             // two buffers of (K tile | V tile), bias table, four arrays of sums
+  const long long item = pa_item(p);
+  if (item >= p.items) return;
+  const int tid = threadIdx.x, lane = tid & 63, wv = wave_uniform(tid >> 6);
+  const int h2 = lane >> 5, lq = lane & 31;
+  const int qb = wave_uniform(p.nblk - 1 - (int)(item % p.nblk));
+  const int unit = wave_uniform((int)(item / p.nblk));
+  const int upb = p.heads / p.gp;
+  const int b = wave_uniform(unit / upb), head0 = wave_uniform((unit - b * upb) * p.gp);
+  const int kvh = wave_uniform(head0 / (p.heads / p.kv_heads));
+  const PRange rg = pa_range(p, b);
+  const int n = rg.n, R2 = 2 * p.R + 1;
+  float* tab = reinterpret_cast<float*>(smem + 4 * PA_TILE);
+  float* dsum = tab + (1 + wv) * R2;
+  const T* Qg = (const T*)p.Q + (size_t)b * p.bsq + head0 * 64;
+  const T* Gg = (const T*)p.dO + (size_t)b * p.bsdo + head0 * 64;
+  const T* Kg = (const T*)p.K + (size_t)b * p.bsk + kvh * 64;
+  const T* Vg = (const T*)p.V + (size_t)b * p.bsv + kvh * 64;
+
+  const int r_base = qb * QB;
+  const int r_last = r_base + QB - 1 < p.rows - 1 ? r_base + QB - 1 : p.rows - 1;
+  const int p0 = wave_uniform(rg.qs + pa_row(p, r_base).i), p1 = wave_uniform(rg.qs + pa_row(p, r_last).i);
+  const PTiles tl = pa_tiles(p, n, p0, p1);
+  const int hi_min = pa_hi(p, n, p0), lo_max = pa_lo(p, p1);
+
+  vec<T, 8> qf[NQ][4], gf[NQ][4];
+  int pos[NQ], ex[NQ];
+  float lse2[NQ], delta[NQ];
+  bool sole[NQ];                                       // the row sees one key: P = 1
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+    const int r = r_base + wv * QW + qi * 32 + lq;
+    const bool ok = r < p.rows;
+    const PRow rw = pa_row(p, ok ? r : p.rows - 1);
+    pos[qi] = rg.qs + (ok ? rw.i : r);                 // (past the last row: any position, its dS is zero)
+    const T* q = Qg + (size_t)rw.i * p.ldq + rw.g * 64;
+    const T* g = Gg + (size_t)rw.i * p.lddo + rw.g * 64;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      qf[qi][ks] = *reinterpret_cast<const vec<T, 8>*>(q + ks * 16 + h2 * 8);
+      gf[qi][ks] = *reinterpret_cast<const vec<T, 8>*>(g + ks * 16 + h2 * 8);
+    }
+    const float l = p.lse[((size_t)b * p.heads + head0 + rw.g) * p.Nq + rw.i];
+    lse2[qi] = !ok || l == PA_NINF ? -PA_NINF : l * PA_LOG2E;
+    const int hi = pa_hi(p, n, pos[qi]), lo0 = pa_lo(p, pos[qi]), lo = lo0 < hi ? lo0 : hi;
+    sole[qi] = hi - lo + (p.sinks < lo ? p.sinks : lo) == 1;
+    ex[qi] = 0;
+    if constexpr (__is_same(T, f16)) {
+      const float amax = pair_max(pa_absmax<T>(gf[qi]));
+      ex[qi] = pa_fit_exp(amax);
+      if (ok && h2 == 0) p.st_amax[(size_t)unit * p.rows + r] = amax;
+    }
+    delta[qi] = 0.f;
+  }
+  float far_l = 0.f, far_r = 0.f;
+  float sum_l = 0.f, sum_r = 0.f;                      // dS of the keys at -R or before, and at R or past it
+  if constexpr (BIAS) {
+    pa_bias_table<NT>(p, head0, tab);
+    for (int i = lane; i < R2; i += 64) dsum[i] = 0.f;
+    block_sync();
+    far_l = tab[0]; far_r = tab[2 * p.R];
+  }
+
+  const int total = tl.na + tl.nb;
+  auto tile_of = [&](int it) STAR_ALWAYS_INLINE { return it < tl.na ? it : it - tl.na + tl.b0; };
+  auto stage = [&](int it, int buf) STAR_ALWAYS_INLINE {
+    const int t = tile_of(it), k0 = t * PA_KT;
+    const int kd = buf * 2 * PA_TILE;
+    const T* kb = Kg + (size_t)k0 * p.ldk;
+    const T* vb = Vg + (size_t)k0 * p.ldv;
+    const bool whole = k0 + PA_KT <= tl.hi && (k0 >= tl.lo || k0 + PA_KT <= tl.sk);
+    if (whole) {
+      pa_stage<NT>(kb, smem, kd, tid, wv, [&](int r, int ch) { return (uint32_t)(r * p.ldk + ch * 8) * 2u; });
+      pa_stage<NT>(vb, smem, kd + PA_TILE, tid, wv, [&](int r, int ch) { return (uint32_t)(r * p.ldv + ch * 8) * 2u; });
+    } else {
+      auto seen = [&](int r) { const int key = k0 + r; return key < tl.hi && (key >= tl.lo || key < tl.sk); };
+      pa_stage<NT>(kb, smem, kd, tid, wv, [&](int r, int ch) { return seen(r) ? (uint32_t)(r * p.ldk + ch * 8) * 2u : GLDS_BUF_OOB; });
+      pa_stage<NT>(vb, smem, kd + PA_TILE, tid, wv, [&](int r, int ch) { return seen(r) ? (uint32_t)(r * p.ldv + ch * 8) * 2u : GLDS_BUF_OOB; });
+    }
+  };
+  const char* kfo[4];                                  // K rows (and V rows, one tile further) as the A operand of S^T and dP^T
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) kfo[ks] = opaque(smem + swz_off(lq, ks * 2 + h2));
+  const char* tfo[2][2];                               // K^T by transposing reads: the A operand of dQ^T = K^T dS^T
+  {
+    const int i = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int db = 0; db < 2; ++db) {
+        const int key = 8 * half + 4 * h2 + (i >> 2), d = 32 * db + 16 * (g & 1) + 4 * (i & 3);
+        tfo[half][db] = opaque(smem + swz_off(key, d >> 3) + (d & 7) * 2);
+      }
+  }
+  f32x16 acc[NQ][2];
+#pragma unroll
+  for (int a = 0; a < NQ; ++a)
+#pragma unroll
+    for (int c2 = 0; c2 < 2; ++c2)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[a][c2][r] = 0.f;
+  float lsum[NQ];
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) lsum[qi] = 0.f;
+
+  // one tile of 64 keys; WALK 0: delta and the row sum, WALK 1: dS and dQ
+  auto tile = [&](int it, int buf, auto walk_tag) STAR_ALWAYS_INLINE {
+    constexpr int WALK = decltype(walk_tag)::value;
+    const int k0 = tile_of(it) * PA_KT;
+    const int bofs = buf * 2 * PA_TILE;
+    const bool masked = !(k0 + PA_KT <= hi_min && (k0 >= lo_max || k0 + PA_KT <= p.sinks));
+    bool near = false, fl = false;
+    float far = 0.f;
+    if constexpr (BIAS) {
+      fl = k0 + PA_KT - 1 - p0 <= -p.R;
+      near = !(fl || k0 - p1 >= p.R);
+      far = fl ? far_l : far_r;
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      f32x16 s[NQ], dp[NQ];
+#pragma unroll
+      for (int qi = 0; qi < NQ; ++qi)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { s[qi][r] = 0.f; dp[qi][r] = 0.f; }
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const vec<T, 8> kf = *reinterpret_cast<const vec<T, 8>*>(kfo[ks] + bofs + kb * 4096);
+        const vec<T, 8> vf = *reinterpret_cast<const vec<T, 8>*>(kfo[ks] + bofs + PA_TILE + kb * 4096);
+#pragma unroll
+        for (int qi = 0; qi < NQ; ++qi) {
+          s[qi] = mfma32<T>(kf, qf[qi][ks], s[qi]);
+          dp[qi] = mfma32<T>(vf, gf[qi][ks], dp[qi]);
+        }
+      }
+      vec<T, 8> ds[NQ][2], dl8[COMP ? NQ : 1][2];
+      // WALK 1: the rounded dS' = 2^ex dS of score r, and dS into the sums by relative position (far tiles: one sum)
+      if (!masked && !near) {
+#pragma unroll
+        for (int qi = 0; qi < NQ; ++qi) {
+          const float off = far - lse2[qi];
+          if constexpr (WALK == 0) {
+            float a0 = 0.f, a1 = 0.f, d0 = 0.f, d1 = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+              const float pa = fast_exp2(__builtin_fmaf(s[qi][r], p.c, off)), pb = fast_exp2(__builtin_fmaf(s[qi][r + 1], p.c, off));
+              a0 += pa; a1 += pb;
+              d0 = __builtin_fmaf(pa, dp[qi][r], d0); d1 = __builtin_fmaf(pb, dp[qi][r + 1], d1);
+            }
+            lsum[qi] += a0 + a1; delta[qi] += d0 + d1;
+          } else {
+            const float pw = pa_pow2(ex[qi]), dl = -delta[qi] * pw;
+            float t0 = 0.f, t1 = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float v = fast_exp2(__builtin_fmaf(s[qi][r], p.c, off)) * __builtin_fmaf(dp[qi][r], pw, dl);
+              if constexpr (BIAS) { if (r & 1) t1 += v; else t0 += v; }
+              T hi16, lo16{};
+              pa_round<T, COMP>(v, hi16, lo16);
+              ds[qi][r >> 3][r & 7] = hi16;
+              if constexpr (COMP) dl8[qi][r >> 3][r & 7] = lo16;
+            }
+            if constexpr (BIAS) {
+              const float t = (t0 + t1) * pa_pow2(-ex[qi]);
+              sum_l += fl ? t : 0.f;
+              sum_r += fl ? 0.f : t;
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int qi = 0; qi < NQ; ++qi) {
+          const int hi = pa_hi(p, n, pos[qi]), lo = pa_lo(p, pos[qi]);
+          const float pw = pa_pow2(ex[qi]), ipw = pa_pow2(-ex[qi]), dl = -delta[qi] * pw;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = k0 + kb * 32 + (r & 3) + 8 * (r >> 2) + 4 * h2;
+            const int rel = key - pos[qi];
+            float bias = far;
+            if constexpr (BIAS) {
+              if (near) { const int i = rel < -p.R ? -p.R : rel > p.R ? p.R : rel; bias = tab[i + p.R]; }
+            }
+            float x = __builtin_fmaf(s[qi][r], p.c, bias - lse2[qi]);
+            if (sole[qi]) x = 0.f;
+            const bool see = !masked || (key < hi && (key >= lo || key < p.sinks));
+            const float pr = see ? fast_exp2(x) : 0.f;
+            if constexpr (WALK == 0) {
+              lsum[qi] += pr;
+              delta[qi] += see ? pr * dp[qi][r] : 0.f;
+            } else {
+              const float v = see ? pr * __builtin_fmaf(dp[qi][r], pw, dl) : 0.f;
+              T hi16, lo16{};
+              pa_round<T, COMP>(v, hi16, lo16);
+              ds[qi][r >> 3][r & 7] = hi16;
+              if constexpr (COMP) dl8[qi][r >> 3][r & 7] = lo16;
+              if constexpr (BIAS) {
+                const float w = v * ipw;
+                sum_l += rel <= -p.R ? w : 0.f;
+                sum_r += rel > -p.R && rel >= p.R ? w : 0.f;
+                // the lanes of one half hold different rows of one key: their words differ; the halves go one after the other
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                  if (h2 == hh && rel > -p.R && rel < p.R) lds_add(dsum + rel + p.R, w);
+                  wave_lds_order();
+                }
+              }
+            }
+          }
+        }
+      }
+      if constexpr (WALK == 1) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int db = 0; db < 2; ++db) {
+            vec<T, 8> kt;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const vec<T, 4> r = lds_read_tr<T>(tfo[half][db] + bofs + (kb * 2 + u) * 2048);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) kt[half * 4 + e] = r[e];
+            }
+#pragma unroll
+            for (int qi = 0; qi < NQ; ++qi) {
+              acc[qi][db] = mfma32<T>(kt, ds[qi][u], acc[qi][db]);
+              if constexpr (COMP) acc[qi][db] = mfma32<T>(kt, dl8[qi][u], acc[qi][db]);
+            }
+          }
+      }
+    }
+  };
+
+  glds_wait();
+  if (total) stage(0, 0);
+  int buf = 0;
+  for (int it = 0; it < total; ++it, buf ^= 1) {
+    glds_wait(); block_sync();
+    stage(it + 1 < total ? it + 1 : 0, buf ^ 1);       // (the second walk's first tile behind the last)
+    tile(it, buf, std::integral_constant<int, 0>{});
+  }
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+    const float l = pair_sum(lsum[qi]), d = pair_sum(delta[qi]);
+    delta[qi] = l > 0.f ? d / l : l == 0.f ? 0.f : l;
+    if (l > 0.f) lse2[qi] += __builtin_log2f(l);
+    const int r = r_base + wv * QW + qi * 32 + lq;
+    if (r < p.rows && h2 == 0) {
+      const size_t at = (size_t)unit * p.rows + r;
+      p.st_lse[at] = lse2[qi];
+      p.st_delta[at] = delta[qi];
+    }
+  }
+  for (int it = 0; it < total; ++it, buf ^= 1) {
+    glds_wait(); block_sync();
+    if (it + 1 < total) stage(it + 1, buf ^ 1);
+    tile(it, buf, std::integral_constant<int, 1>{});
+  }
+#pragma unroll
+  for (int qi = 0; qi < NQ; ++qi) {
+    const int r = r_base + wv * QW + qi * 32 + lq;
+    const bool ok = r < p.rows;
+    const PRow rw = pa_row(p, ok ? r : p.rows - 1);
+    pa_store_row<T>(acc[qi], p.scale * pa_pow2(-ex[qi]), (T*)p.dQ + (size_t)b * p.bsdq + (size_t)rw.i * p.lddq + (head0 + rw.g) * 64, ok);
+  }
+  if constexpr (BIAS) {
+    const float tl2 = wave_sum(sum_l), tr2 = wave_sum(sum_r);
+    if (lane == 0) {
+      if (p.R > 0) { dsum[0] = tl2; dsum[2 * p.R] = tr2; }
+      else dsum[0] = tl2 + tr2;
+    }
+    block_sync();
+    float* out = p.dsum + ((size_t)unit * p.nblk + qb) * R2;
+    for (int i = tid; i < R2; i += NT) out[i] = (tab[R2 + i] + tab[2 * R2 + i]) + (tab[3 * R2 + i] + tab[4 * R2 + i]);
+  }
+}
+
+// the part of a key block that a slot of a unit stands for
+struct PSlot { int kblk, part, parts; };
+STAR_DEV PSlot pa_slot(const PAttnParams& p, int slot) {
+  const int first = p.sblk * p.split_s;
+  if (slot < first) { const int k = wave_uniform(slot / p.split_s); return PSlot{k, slot - k * p.split_s, p.split_s}; }
+  const int k = wave_uniform((slot - first) / p.split_n);
+  return PSlot{p.sblk + k, slot - first - k * p.split_n, p.split_n};
+}
+
+template <class T, int BIAS, int COMP>
+STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256, 2)
+pattn_dkdv_kernel(const PAttnParams p) {
+  constexpr int NT = 256, KB = 128, QT = 64;           // keys per workgroup, query rows per tile
+  constexpr int SHIFT = __is_same(T, f16) ? 10 : 0;    // P is rounded as 2^SHIFT P
+  constexpr int ROWB = QT * 12 + 16, BUF = 2 * PA_TILE + ROWB;   // Q tile | dO tile | off[64] | delta[64] | pos[64] | exponent
+  char* smem = dyn_smem();                             // two such buffers, then the bias table
+  const long long item = pa_item(p);
+  if (item >= p.items) return;
+  const int tid = threadIdx.x, lane = tid & 63, wv = wave_uniform(tid >> 6);
+  const int h2 = lane >> 5, lq = lane & 31;
+  const PSlot sl = pa_slot(p, wave_uniform((int)(item % p.nblk)));    // nblk: slots per unit
+  const int kblk = sl.kblk;
+  const int ku = wave_uniform((int)(item / p.nblk));   // (sequence, K / V head); one sequence where the batch shares K and V
+  const int kb0 = wave_uniform(ku / p.kv_heads), kvh = ku - kb0 * p.kv_heads;
+  const bool shared = p.batch > 1 && p.bsk == 0 && p.bsv == 0;
+  const int j0 = kblk * KB, jw = j0 + wv * 32, key = jw + lq;
+  float* tab = reinterpret_cast<float*>(smem + 2 * BUF);
+
+  vec<T, 8> kf[4], vf[4];
+  {
+    const int nk = shared ? p.Nk : pa_range(p, kb0).n;
+    const T* K = (const T*)p.K + (size_t)kb0 * p.bsk + kvh * 64 + (size_t)(key < nk ? key : 0) * p.ldk;
+    const T* V = (const T*)p.V + (size_t)kb0 * p.bsv + kvh * 64 + (size_t)(key < nk ? key : 0) * p.ldv;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { kf[ks][e] = from_f32<T>(0.f); vf[ks][e] = from_f32<T>(0.f); }
+      if (key < nk) {
+        kf[ks] = *reinterpret_cast<const vec<T, 8>*>(K + ks * 16 + h2 * 8);
+        vf[ks] = *reinterpret_cast<const vec<T, 8>*>(V + ks * 16 + h2 * 8);
+      }
+    }
+  }
+  f32x16 dk[2], dv[2];
+#pragma unroll
+  for (int c2 = 0; c2 < 2; ++c2)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) { dk[c2][r] = 0.f; dv[c2][r] = 0.f; }
+
+  const char* afo[4];                                  // Q rows (and dO rows, one tile further) as the A operand of S and dP
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) afo[ks] = opaque(smem + swz_off(lq, ks * 2 + h2));
+  const char* tfo[2][2];                               // Q^T (and dO^T) by transposing reads: the A operands of dK^T and dV^T
+  {
+    const int i = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int db = 0; db < 2; ++db) {
+        const int q = 8 * half + 4 * h2 + (i >> 2), d = 32 * db + 16 * (g & 1) + 4 * (i & 3);
+        tfo[half][db] = opaque(smem + swz_off(q, d >> 3) + (d & 7) * 2);
+      }
+  }
+
+  const int G = wave_uniform(p.heads / p.kv_heads), subs = wave_uniform(G / p.gp), upb = wave_uniform(p.heads / p.gp);
+  const int nb = shared ? p.batch : 1;
+  // the tiles [t0, t1) of the rows of sequence b that see some key of the block
+  auto tiles_of = [&](const PRange& rg, int& t0, int& t1) STAR_ALWAYS_INLINE {
+    const int j1 = j0 + KB - 1 < rg.n - 1 ? j0 + KB - 1 : rg.n - 1;
+    int i0 = j0 - p.right - rg.qs, i1 = j0 < p.sinks ? p.Nq : j1 + p.left - rg.qs + 1;
+    i0 = i0 < 0 ? 0 : i0; i1 = i1 > p.Nq ? p.Nq : i1;
+    t0 = 0; t1 = 0;
+    if (j0 < rg.n && i0 < i1) { t0 = (int)((long long)i0 * p.gp / QT); t1 = (int)(((long long)i1 * p.gp + QT - 1) / QT); }
+  };
+  // this part's share of all tiles, counted over the heads of the group and the sequences one after the other
+  long long first = 0, last = 0x7fffffffffffLL;
+  if (sl.parts > 1) {
+    long long all = 0;
+    for (int b = shared ? 0 : kb0; b < (shared ? p.batch : kb0 + 1); ++b) {
+      int t0, t1;
+      tiles_of(pa_range(p, b), t0, t1);
+      all += (long long)(t1 - t0) * subs;
+    }
+    first = all * sl.part / sl.parts; last = all * (sl.part + 1) / sl.parts;
+  }
+  long long done = 0;                                  // tiles before the current head's
+  int E = 40;                                          // f16: dK is summed as 2^E dK
+  for (int w = 0; w < nb * subs; ++w) {
+    const int b = shared ? wave_uniform(w / subs) : kb0, sub = shared ? w - b * subs : w;
+    const int head0 = kvh * G + sub * p.gp, unit = b * upb + kvh * subs + sub;
+    const PRange rg = pa_range(p, b);
+    const int n = rg.n;
+    int t0, t1;
+    tiles_of(rg, t0, t1);
+    const long long here = done;
+    done += t1 - t0;
+    if (sl.parts > 1) {
+      const long long lo = first - here, hi = last - here;
+      const int base = t0, cnt = t1 - t0;
+      t0 = wave_uniform(base + (int)(lo < 0 ? 0 : lo > cnt ? cnt : lo)); t1 = wave_uniform(base + (int)(hi < 0 ? 0 : hi > cnt ? cnt : hi));
+    }
+    if (t0 >= t1) continue;
+    const T* Qg = (const T*)p.Q + (size_t)b * p.bsq + head0 * 64;
+    const T* Gg = (const T*)p.dO + (size_t)b * p.bsdo + head0 * 64;
+    float far_l = 0.f, far_r = 0.f;
+    if constexpr (BIAS) {
+      block_sync();                                    // the last tile's readers are done with the table
+      pa_bias_table<NT>(p, head0, tab);
+      block_sync();
+      far_l = tab[0]; far_r = tab[2 * p.R];
+    } else block_sync();
+
+    auto bounds = [&](int t, int& pa, int& pb) STAR_ALWAYS_INLINE {    // positions of a tile's first and last row
+      const int rl = t * QT + QT - 1 < p.rows - 1 ? t * QT + QT - 1 : p.rows - 1;
+      pa = wave_uniform(rg.qs + pa_row(p, t * QT).i); pb = wave_uniform(rg.qs + pa_row(p, rl).i);
+    };
+    auto stage = [&](int t, int buf) STAR_ALWAYS_INLINE {
+      const int d = buf * BUF;
+      const int r0 = t * QT, i_first = wave_uniform(pa_row(p, r0).i);
+      const T* qb = Qg + (size_t)i_first * p.ldq;
+      const T* gb = Gg + (size_t)i_first * p.lddo;
+      auto at = [&](int r, int ch, int ld) {
+        const PRow rw = pa_row(p, r0 + r);
+        return r0 + r < p.rows ? (uint32_t)((rw.i - i_first) * ld + rw.g * 64 + ch * 8) * 2u : GLDS_BUF_OOB;
+      };
+      pa_stage<NT>(qb, smem, d, tid, wv, [&](int r, int ch) { return at(r, ch, p.ldq); });
+      pa_stage<NT>(gb, smem, d + PA_TILE, tid, wv, [&](int r, int ch) { return at(r, ch, p.lddo); });
+    };
+    // a row's statistics: loaded by the first wave a tile ahead, written to LDS when the tile's turn comes
+    float x_lse = 0.f, x_delta = 0.f, x_amax = 0.f;
+    auto load_rows = [&](int t) STAR_ALWAYS_INLINE {
+      const int r = t * QT + tid;
+      x_lse = -PA_NINF; x_delta = 0.f; x_amax = 0.f;
+      if (tid < QT && r < p.rows) {
+        const size_t a = (size_t)unit * p.rows + r;
+        x_lse = p.st_lse[a]; x_delta = p.st_delta[a];
+        if constexpr (SHIFT) x_amax = p.st_amax[a];
+      }
+    };
+    int e_row = E;                                       // (first wave) the exponent up to the tile being written
+    auto write_rows = [&](int t, int buf) STAR_ALWAYS_INLINE {
+      if (wv) return;
+      float* o = reinterpret_cast<float*>(smem + buf * BUF + 2 * PA_TILE);
+      float far = 0.f;
+      if constexpr (BIAS) {
+        int pa, pb;
+        bounds(t, pa, pb);
+        if (j0 + KB - 1 - pa <= -p.R) far = far_l;
+        else if (j0 - pb >= p.R) far = far_r;
+      }
+      if constexpr (SHIFT) {
+        const float m = wave_max(x_amax);
+        if (m > 0.f) { const int e = pa_fit_exp(m); if (e < e_row) e_row = e; }
+      }
+      o[tid] = far - x_lse + (float)SHIFT;
+      o[64 + tid] = SHIFT ? x_delta * pa_pow2(e_row - SHIFT) : x_delta;
+      reinterpret_cast<int*>(o)[128 + tid] = rg.qs + pa_row(p, t * QT + tid).i;
+      if (SHIFT && tid == 0) reinterpret_cast<int*>(o)[192] = e_row;
+    };
+
+    auto tile = [&](int t, int buf) STAR_ALWAYS_INLINE {
+      int pa, pb;
+      bounds(t, pa, pb);
+      const int jl = jw + 31;
+      const int bofs = buf * BUF;
+      const float* o = reinterpret_cast<const float*>(smem + bofs + 2 * PA_TILE);
+      float pw = 1.f;
+      if constexpr (SHIFT) {
+        const int e = wave_uniform(reinterpret_cast<const int*>(o)[192]);
+        if (e != E) {                                    // larger gradients than so far: lower the common exponent
+          const float f = pa_pow2(e - E);
+#pragma unroll
+          for (int c2 = 0; c2 < 2; ++c2)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dk[c2][r] *= f;
+          E = e;
+        }
+        pw = pa_pow2(E - SHIFT);
+      }
+      if (jw >= n || jw > pb + p.right || (jl < pa - p.left && jw >= p.sinks)) return;   // no row of the tile sees a key of the wave
+      const bool masked = !(jl < n && jl <= pa + p.right && (jw >= pb - p.left || jl < p.sinks));
+      const bool near = BIAS ? !(j0 + KB - 1 - pa <= -p.R || j0 - pb >= p.R) : false;
+#pragma unroll
+      for (int qs = 0; qs < 2; ++qs) {
+        f32x16 s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const vec<T, 8> a = *reinterpret_cast<const vec<T, 8>*>(afo[ks] + bofs + qs * 4096);
+          const vec<T, 8> g = *reinterpret_cast<const vec<T, 8>*>(afo[ks] + bofs + PA_TILE + qs * 4096);
+          s = mfma32<T>(a, kf[ks], s);
+          dp = mfma32<T>(g, vf[ks], dp);
+        }
+        vec<T, 8> pf[2], df[2], pl[2], dl8[2];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {                    // rows 8 g + 4 h2 + (0 .. 3) of the 32
+          const int row = qs * 32 + 8 * g + 4 * h2;
+          const f32x4 off = *reinterpret_cast<const f32x4*>(o + row), dl = *reinterpret_cast<const f32x4*>(o + 64 + row);
+          if (!masked && !near) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float pr = fast_exp2(__builtin_fmaf(s[4 * g + e], p.c, off[e]));
+              const float v = pr * (SHIFT ? __builtin_fmaf(dp[4 * g + e], pw, -dl[e]) : dp[4 * g + e] - dl[e]);
+              T a, al{}, d, dl_{};
+              pa_round<T, COMP>(pr, a, al);
+              pa_round<T, COMP>(v, d, dl_);
+              pf[g >> 1][(g & 1) * 4 + e] = a; df[g >> 1][(g & 1) * 4 + e] = d;
+              if constexpr (COMP) { pl[g >> 1][(g & 1) * 4 + e] = al; dl8[g >> 1][(g & 1) * 4 + e] = dl_; }
+            }
+          } else {
+            const vec<int, 4> ps = *reinterpret_cast<const vec<int, 4>*>(reinterpret_cast<const int*>(o) + 128 + row);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int rel = key - ps[e];
+              float of = off[e];
+              if constexpr (BIAS) {
+                if (near) { const int i = rel < -p.R ? -p.R : rel > p.R ? p.R : rel; of += tab[i + p.R]; }
+              }
+              const bool see = !masked || (key < n && rel <= p.right && (rel >= -p.left || key < p.sinks));
+              const float pr = see ? fast_exp2(__builtin_fmaf(s[4 * g + e], p.c, of)) : 0.f;
+              const float v = see ? pr * (SHIFT ? __builtin_fmaf(dp[4 * g + e], pw, -dl[e]) : dp[4 * g + e] - dl[e]) : 0.f;
+              T a, al{}, d, dl_{};
+              pa_round<T, COMP>(pr, a, al);
+              pa_round<T, COMP>(v, d, dl_);
+              pf[g >> 1][(g & 1) * 4 + e] = a; df[g >> 1][(g & 1) * 4 + e] = d;
+              if constexpr (COMP) { pl[g >> 1][(g & 1) * 4 + e] = al; dl8[g >> 1][(g & 1) * 4 + e] = dl_; }
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int db = 0; db < 2; ++db) {
+            vec<T, 8> qt, gt;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const vec<T, 4> a = lds_read_tr<T>(tfo[half][db] + bofs + (qs * 2 + u) * 2048);
+              const vec<T, 4> g = lds_read_tr<T>(tfo[half][db] + bofs + PA_TILE + (qs * 2 + u) * 2048);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) { qt[half * 4 + e] = a[e]; gt[half * 4 + e] = g[e]; }
+            }
+            dv[db] = mfma32<T>(gt, pf[u], dv[db]);
+            dk[db] = mfma32<T>(qt, df[u], dk[db]);
+            if constexpr (COMP) {
+              dv[db] = mfma32<T>(gt, pl[u], dv[db]);
+              dk[db] = mfma32<T>(qt, dl8[u], dk[db]);
+            }
+          }
+      }
+    };
+
+    load_rows(t0);
+    glds_wait();                                         // no compiler-visible load in flight beside the hand-written DMA's first use
+    stage(t0, 0);
+    for (int t = t0; t < t1; ++t) {
+      const int buf = (t - t0) & 1;
+      write_rows(t, buf);
+      glds_wait(); block_sync();
+      if (t + 1 < t1) { load_rows(t + 1); stage(t + 1, buf ^ 1); }
+      tile(t, buf);
+    }
+  }
+
+  const float mk = p.scale * (SHIFT ? pa_pow2(-E) : 1.f), mv = pa_pow2(-SHIFT);
+  if (sl.parts > 1) {
+    // [unit][slot][key][dK 64 | dV 64]; only blocks in parts have slots there
+    const int per = p.split_n > 1 ? p.nblk : p.sblk * p.split_s;
+    float* o = p.part + (((size_t)ku * per + (int)(item % p.nblk)) * KB + wv * 32 + lq) * 128;
+#pragma unroll
+    for (int db = 0; db < 2; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f32x4 a, c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { a[e] = dk[db][g * 4 + e] * mk; c[e] = dv[db][g * 4 + e] * mv; }
+        *reinterpret_cast<f32x4*>(o + 32 * db + 8 * g + 4 * h2) = a;
+        *reinterpret_cast<f32x4*>(o + 64 + 32 * db + 8 * g + 4 * h2) = c;
+      }
+    return;
+  }
+  const int ob = shared ? 0 : kb0;
+  const bool ok = key < p.Nk;
+  pa_store_row<T>(dk, mk, (T*)p.dK + (size_t)ob * p.bsdk + (size_t)(ok ? key : 0) * p.lddk + kvh * 64, ok);
+  pa_store_row<T>(dv, mv, (T*)p.dV + (size_t)ob * p.bsdv + (size_t)(ok ? key : 0) * p.lddv + kvh * 64, ok);
+}
+
+// adds the parts of the key blocks that were split, in their order: one workgroup per block, a thread per eight values
+template <class T>
+STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256)
+pattn_dkdv_join_kernel(const PAttnParams p) {
+  const int first = p.sblk * p.split_s;                // slots of the first blocks
+  const int nsplit = p.split_n > 1 ? p.sblk + (p.nblk - first) / p.split_n : p.sblk;      // blocks in parts (all, or those of the first tokens)
+  const int ku = blockIdx.x / nsplit, k = blockIdx.x - ku * nsplit;
+  const int parts = k < p.sblk ? p.split_s : p.split_n;
+  const int slot = k < p.sblk ? k * p.split_s : first + (k - p.sblk) * p.split_n;
+  const int per = p.split_n > 1 ? p.nblk : first;
+  const int b = ku / p.kv_heads, kvh = ku - b * p.kv_heads;
+  const float* src = p.part + ((size_t)ku * per + slot) * 128 * 128;
+  for (int i = threadIdx.x; i < 128 * 16; i += 256) {
+    const int row = i >> 4, c = (i & 15) * 8, key = k * 128 + row;
+    if (key >= p.Nk) continue;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    for (int q = 0; q < parts; ++q) {
+      const f32x4* a = reinterpret_cast<const f32x4*>(src + ((size_t)q * 128 + row) * 128 + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { v[e] += a[0][e]; v[4 + e] += a[1][e]; }
+    }
+    vec<T, 8> o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = from_f32<T>(v[e]);
+    T* dst = c < 64 ? (T*)p.dK + (size_t)b * p.bsdk + (size_t)key * p.lddk + kvh * 64 + c : (T*)p.dV + (size_t)b * p.bsdv + (size_t)key * p.lddv + kvh * 64 + c - 64;
+    *reinterpret_cast<vec<T, 8>*>(dst) = o;
+  }
+}
+
+// dtable[k][h]: the sums of a head's row blocks by relative position, in double and in a fixed order, then by bucket
+struct PDTableParams { const float* dsum; const int* buckets; float* dtable; int batch, heads, nblk, R, num_buckets; };
+STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256)
+pattn_dtable_kernel(const PDTableParams p) {
+  double* rel = reinterpret_cast<double*>(dyn_smem());
+  const int h = blockIdx.x, R2 = 2 * p.R + 1;
+  for (int i = threadIdx.x; i < R2; i += 256) {
+    double s = 0.0;
+    for (int b = 0; b < p.batch; ++b) {
+      const float* d = p.dsum + ((size_t)b * p.heads + h) * p.nblk * R2 + i;
+#pragma unroll 4
+      for (int q = 0; q < p.nblk; ++q) s += (double)d[(size_t)q * R2];
+    }
+    rel[i] = s;
+  }
+  block_sync();
+  for (int k = threadIdx.x; k < p.num_buckets; k += 256) {
+    double s = 0.0;
+    for (int i = 0; i < R2; ++i) {
+      int c = p.buckets[i];
+      c = c < 0 ? 0 : c >= p.num_buckets ? p.num_buckets - 1 : c;
+      if (c == k) s += rel[i];
+    }
+    p.dtable[(size_t)k * p.heads + h] = (float)s;
+  }
+}
+
+}  // namespace star

@@ -37,6 +37,28 @@ class AttnDesc(ctypes.Structure):
     ]
 
 
+class PosAttnDesc(ctypes.Structure):
+    _fields_ = [
+        ("Q", ctypes.c_void_p), ("K", ctypes.c_void_p), ("V", ctypes.c_void_p), ("O", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("ldq", ctypes.c_int32), ("ldk", ctypes.c_int32), ("ldv", ctypes.c_int32), ("ldo", ctypes.c_int32),
+        ("bsq", ctypes.c_int64), ("bsk", ctypes.c_int64), ("bsv", ctypes.c_int64), ("bso", ctypes.c_int64),
+        ("Nq", ctypes.c_int32), ("Nk", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("batch", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("left", ctypes.c_int32), ("right", ctypes.c_int32), ("sinks", ctypes.c_int32),
+        ("num_buckets", ctypes.c_int32), ("bias_range", ctypes.c_int32),
+        ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p), ("bias_table", ctypes.c_void_p), ("bias_buckets", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class PosAttnGrads(ctypes.Structure):
+    _fields_ = [
+        ("dO", ctypes.c_void_p), ("dQ", ctypes.c_void_p), ("dK", ctypes.c_void_p), ("dV", ctypes.c_void_p),
+        ("lddo", ctypes.c_int32), ("lddq", ctypes.c_int32), ("lddk", ctypes.c_int32), ("lddv", ctypes.c_int32),
+        ("bsdo", ctypes.c_int64), ("bsdq", ctypes.c_int64), ("bsdk", ctypes.c_int64), ("bsdv", ctypes.c_int64),
+        ("dbias_table", ctypes.c_void_p),
+    ]
+
+
 class TAttnDesc(ctypes.Structure):
     _fields_ = [
         ("Q", ctypes.c_void_p), ("K", ctypes.c_void_p), ("V", ctypes.c_void_p), ("O", ctypes.c_void_p),
@@ -128,6 +150,13 @@ class Library:
         self.layer_norm = _sig(c, "star_layer_norm", i32, vp, vp, i32, vp, i32, vp, vp, i32, i32, f32, i32, vp, vp, i32, i32)
         self.layer_norm_rowab_from_partials = _sig(c, "star_layer_norm_rowab_from_partials", i32, vp, vp, i32, vp, i32, i32, ctypes.c_float, i32, vp, vp, i32, i32)
         self.layer_norm_rowab = _sig(c, "star_layer_norm_rowab", i32, vp, vp, i32, vp, i32, i32, f32, i32, vp, vp, i32, i32)
+        self.layer_norm_train = _sig(c, "star_layer_norm_train", i32, vp, vp, i64, vp, i64, vp, vp, vp, i32, i32, f32)
+        self.layer_norm_bwd_workspace = _sig(c, "star_layer_norm_bwd_workspace", sz, vp, i32, i32)
+        self.layer_norm_bwd = _sig(c, "star_layer_norm_bwd", i32, vp, vp, i64, vp, i64, vp, vp, vp, i64, vp, vp, i32, i32, vp, sz)
+        self.pos_attn_workspace = _sig(c, "star_pos_attn_workspace", sz, vp, ctypes.POINTER(PosAttnDesc), i32)
+        self.pos_attn_fwd = _sig(c, "star_pos_attn_fwd", i32, vp, ctypes.POINTER(PosAttnDesc))
+        self.pos_attn_bwd = _sig(c, "star_pos_attn_bwd", i32, vp, ctypes.POINTER(PosAttnDesc), ctypes.POINTER(PosAttnGrads))
+        self.rel_buckets = _sig(c, "star_rel_buckets", i32, i32, i32, i32, ctypes.POINTER(ctypes.c_int32))
         self.concat_add = _sig(c, "star_concat_add", i32, vp, vp, vp, vp, vp, i32, i32, i32)
         self.add = _sig(c, "star_add", i32, vp, vp, vp, vp, i64)
         self.stem_im2col = _sig(c, "star_stem_im2col", i32, vp, vp, vp, i32, i32, i32, i32)
@@ -158,6 +187,10 @@ def default_library():
 
 def _ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 def device_index(device):
@@ -438,6 +471,203 @@ class Context:
         self._check(self.lib.layer_norm_rowab_from_partials(self.h, _ptr(partial), parts, _ptr(rowab), rows, C, float(eps), mode, _ptr(gate_w),
                                                             _ptr(maps), H, W), "layer_norm_rowab_from_partials")
         return maps if mode == LN_STATS_ONLY else rowab
+
+    # ------------------------------------------------------------------ training and position-dependent attention
+    # These calls follow torch's current stream, allocate what they return and their workspaces there, and leave the arena alone: they may
+    # be captured into graphs, and calls on several streams do not share scratch memory.
+    def _rows(self, t, what, shape=None, dtype=None):
+        """rows of a [..., C] tensor with unit column stride: checked, and with a stride that says something where there is one row"""
+        if not isinstance(t, torch.Tensor):
+            raise StarError(f"{what} must be a tensor")
+        self._chk_tensor(t, dtype or self.dtype)
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise StarError(f"{what} must be {list(shape)}, got {list(t.shape)}")
+        if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise StarError(f"{what} must have unit stride in its last dimension")
+        return t
+
+    def _vec_f32(self, t, n, what):
+        if t is None:
+            return
+        self._chk_tensor(t, torch.float32)
+        if tuple(t.shape) != (n,) or not t.is_contiguous():
+            raise StarError(f"{what} must be a contiguous fp32 [{n}]")
+
+    @staticmethod
+    def _ld(t, dim, width):
+        """stride of `dim`; a dimension of one row has whatever stride torch left there"""
+        ld = t.stride(dim) if t.shape[dim] > 1 and t.numel() else width
+        if dim == t.dim() - 2 and ld >= 2 ** 31:
+            raise StarError(f"a row stride of {ld} elements is too large")
+        return ld
+
+    def _follow_stream(self):
+        if not self.lib.is_hostemu:
+            self._check(self.lib.set_stream(self.h, torch.cuda.current_stream(self.device_index).cuda_stream), "set_stream")
+
+    def layer_norm_train(self, x, gamma=None, beta=None, eps=1e-5, out=None):
+        """LayerNorm over the last dimension of x: [rows, C] that keeps its row statistics -> (y, stats fp32 [rows, 2] = (mean, rstd)).
+        gamma, beta: fp32 [C] or None.  Any C up to 16384; out may be x."""
+        self._rows(x, "x")
+        if x.dim() != 2 or x.shape[0] >= 2 ** 31:
+            raise StarError("x must be [rows, C], with fewer than 2^31 rows")
+        rows, C = x.shape
+        self._vec_f32(gamma, C, "gamma")
+        self._vec_f32(beta, C, "beta")
+        self._follow_stream()
+        if out is None:
+            out = torch.empty(rows, C, dtype=self.dtype, device=self.torch_device)
+        else:
+            self._rows(out, "out", (rows, C))
+        stats = torch.empty(rows, 2, dtype=torch.float32, device=self.torch_device)
+        self._check(self.lib.layer_norm_train(self.h, x.data_ptr(), self._ld(x, 0, C), out.data_ptr(), self._ld(out, 0, C), _addr(gamma), _addr(beta),
+                                              stats.data_ptr(), rows, C, eps), "layer_norm_train")
+        return out, stats
+
+    def layer_norm_backward(self, dy, x, stats, gamma=None, dx=None, need_weights=True):
+        """backward pass of layer_norm_train -> (dx, dgamma, dbeta); need_weights=False: (dx, None, None).  dx may be x or dy."""
+        self._rows(x, "x")
+        if x.dim() != 2 or x.shape[0] >= 2 ** 31:
+            raise StarError("x must be [rows, C], with fewer than 2^31 rows")
+        rows, C = x.shape
+        self._rows(dy, "dy", (rows, C))
+        self._rows(stats, "stats", (rows, 2), torch.float32)
+        if not stats.is_contiguous():
+            raise StarError("stats must be contiguous")
+        self._vec_f32(gamma, C, "gamma")
+        self._follow_stream()
+        if dx is None:
+            dx = torch.empty(rows, C, dtype=self.dtype, device=self.torch_device)
+        else:
+            self._rows(dx, "dx", (rows, C))
+        dgamma = dbeta = ws = None
+        nbytes = 0
+        if need_weights:
+            dgamma = torch.empty(C, dtype=torch.float32, device=self.torch_device)
+            dbeta = torch.empty(C, dtype=torch.float32, device=self.torch_device)
+            nbytes = self.lib.layer_norm_bwd_workspace(self.h, rows, C)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.torch_device) if nbytes else None
+        self._check(self.lib.layer_norm_bwd(self.h, dy.data_ptr(), self._ld(dy, 0, C), x.data_ptr(), self._ld(x, 0, C), stats.data_ptr(), _addr(gamma),
+                                            dx.data_ptr(), self._ld(dx, 0, C), _addr(dgamma), _addr(dbeta), rows, C, _addr(ws), nbytes), "layer_norm_bwd")
+        return dx, dgamma, dbeta
+
+    def rel_buckets(self, num_buckets=32, max_distance=128, bidirectional=True):
+        """bucket of each relative position j - p = -max_distance .. max_distance (int32 [2 * max_distance + 1] on the device), for
+        pos_attention's bias; positions further off share the end's bucket"""
+        n = 2 * int(max_distance) + 1
+        buf = (ctypes.c_int32 * max(n, 1))()
+        if n < 3 or self.lib.rel_buckets(int(num_buckets), int(max_distance), int(bool(bidirectional)), buf):
+            raise StarError(f"rel_buckets: {num_buckets} buckets over a distance of {max_distance} do not make a scheme")
+        return torch.tensor(list(buf), dtype=torch.int32).to(self.torch_device)
+
+    def _pos_desc(self, q, k, v, heads, kv_heads, scale, window, sinks, causal, q_start, kv_len, bias):
+        kv_heads = heads if kv_heads is None else kv_heads
+        for t, what in ((q, "q"), (k, "k"), (v, "v")):
+            self._rows(t, what)
+            if t.dim() != 3:
+                raise StarError(f"{what} must be [batch, tokens, heads * 64]")
+        B, Nq, _ = q.shape
+        Nk = k.shape[1]
+        if heads < 1 or kv_heads < 1 or heads % kv_heads:
+            raise StarError("kv_heads must divide heads")
+        if q.shape[2] != heads * 64 or k.shape[2] != kv_heads * 64 or v.shape[2] != kv_heads * 64:
+            raise StarError(f"q must be [B, Nq, {heads * 64}], k and v [B or 1, Nk, {kv_heads * 64}]")
+        if v.shape[1] != Nk or k.shape[0] != v.shape[0] or k.shape[0] not in (B, 1):
+            raise StarError("k and v must have the same keys, for every sequence or once for all")
+        d = PosAttnDesc()
+        d.Q, d.K, d.V = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        d.ldq, d.ldk, d.ldv = (self._ld(t, 1, t.shape[2]) for t in (q, k, v))
+        d.bsq = self._ld(q, 0, 0)
+        d.bsk, d.bsv = (self._ld(t, 0, 0) for t in (k, v))
+        if B > 1 and k.shape[0] == B and Nk and (d.bsk == 0) != (d.bsv == 0):
+            raise StarError("k and v must both be expanded over the batch, or neither")
+        if max(Nq, Nk) > 2 ** 28 or heads * max(Nq, 1) >= 2 ** 31 or B * heads >= 2 ** 31:
+            raise StarError("too many rows")
+        d.Nq, d.Nk, d.heads, d.kv_heads, d.batch = Nq, Nk, heads, kv_heads, B
+        d.scale = float(scale if scale is not None else 64 ** -0.5)
+        left, right = (-1, -1) if window is None else window
+        left, right = (-1 if s is None else max(-1, min(int(s), 2 ** 30)) for s in (left, right))
+        if causal:
+            right = 0
+        d.left, d.right, d.sinks = left, right, max(-1, min(int(sinks), 2 ** 28))
+        for t, what in ((q_start, "q_start"), (kv_len, "kv_len")):
+            if t is not None:
+                self._chk_tensor(t, torch.int32)
+                if tuple(t.shape) != (B,) or not t.is_contiguous():
+                    raise StarError(f"{what} must be a contiguous int32 [{B}]")
+        d.q_start = q_start.data_ptr() if q_start is not None else None
+        d.kv_len = kv_len.data_ptr() if kv_len is not None else None
+        if bias is not None:
+            table, buckets = bias
+            self._chk_tensor(table, torch.float32)
+            self._chk_tensor(buckets, torch.int32)
+            if table.dim() != 2 or table.shape[1] != heads or not table.is_contiguous():
+                raise StarError(f"the bias table must be a contiguous fp32 [buckets, {heads}]")
+            if buckets.dim() != 1 or buckets.shape[0] % 2 == 0 or not buckets.is_contiguous():
+                raise StarError("the bias buckets must be a contiguous int32 [2 * range + 1]")
+            d.bias_table, d.bias_buckets = table.data_ptr(), buckets.data_ptr()
+            d.num_buckets, d.bias_range = table.shape[0], buckets.shape[0] // 2
+        return d
+
+    def _pos_workspace(self, d, backward):
+        d.workspace_bytes = self.lib.pos_attn_workspace(self.h, ctypes.byref(d), int(backward))
+        ws = torch.empty(d.workspace_bytes, dtype=torch.uint8, device=self.torch_device) if d.workspace_bytes else None
+        d.workspace = ws.data_ptr() if ws is not None else None
+        return ws
+
+    def pos_attention(self, q, k, v, heads, kv_heads=None, *, scale=None, window=None, sinks=0, causal=False, q_start=None, kv_len=None, bias=None,
+                      out=None, return_lse=False):
+        """Attention with a sliding window, first tokens that stay visible, lengths and positions per sequence, grouped heads and a learned
+        relative position bias by buckets (star_pos_attn_fwd).  q: [B, Nq, heads*64]; k, v: [B or 1, Nk, kv_heads*64]; views with a row
+        stride are fine (fused projections, caches).
+          window = (left, right): keys at most that far before / after the query's position (None or negative: no limit); causal: right = 0
+          sinks: the first keys, visible past the left end of the window too
+          q_start, kv_len: int32 [B] on the device: position of each sequence's row 0 (default Nk - Nq) and its keys in hand (default Nk)
+          bias = (table fp32 [buckets, heads], buckets int32 [2 R + 1] of rel_buckets())
+        -> [B, Nq, heads*64], with return_lse also log sum exp of the scores, fp32 [B, heads, Nq].  A row that sees no key: 0 and -inf."""
+        d = self._pos_desc(q, k, v, heads, kv_heads, scale, window, sinks, causal, q_start, kv_len, bias)
+        B, Nq = q.shape[:2]
+        self._follow_stream()
+        if out is None:
+            out = torch.empty(B, Nq, heads * 64, dtype=self.dtype, device=self.torch_device)
+        else:
+            self._rows(out, "out", (B, Nq, heads * 64))
+        d.O, d.ldo, d.bso = out.data_ptr(), self._ld(out, 1, heads * 64), self._ld(out, 0, 0)
+        lse = torch.empty(B, heads, Nq, dtype=torch.float32, device=self.torch_device) if return_lse else None
+        d.lse = lse.data_ptr() if lse is not None else None
+        ws = self._pos_workspace(d, False)      # held until the call is queued
+        self._check(self.lib.pos_attn_fwd(self.h, ctypes.byref(d)), "pos_attn_fwd")
+        del ws
+        return (out, lse) if return_lse else out
+
+    def pos_attention_backward(self, dout, q, k, v, lse, heads, kv_heads=None, *, scale=None, window=None, sinks=0, causal=False, q_start=None,
+                               kv_len=None, bias=None, dq=None, dk=None, dv=None):
+        """backward pass of pos_attention, with the arguments and the lse of the forward call -> (dq, dk, dv, dtable); dtable (fp32
+        [buckets, heads]) is None without a bias.  Gradients have the shapes of q, k, v: where all sequences share k and v, sums over them."""
+        d = self._pos_desc(q, k, v, heads, kv_heads, scale, window, sinks, causal, q_start, kv_len, bias)
+        B, Nq = q.shape[:2]
+        self._rows(dout, "dout", q.shape)
+        self._rows(lse, "lse", (B, heads, Nq), torch.float32)
+        if not lse.is_contiguous():
+            raise StarError("lse must be contiguous")
+        if B > 1 and k.shape[0] == B and k.numel() and d.bsk == 0:
+            raise StarError("k and v are expanded over the batch: pass them as [1, Nk, ...], their gradients are sums over the batch")
+        self._follow_stream()
+        dq, dk, dv = (torch.empty(t.shape, dtype=self.dtype, device=self.torch_device) if g is None else g for t, g in ((q, dq), (k, dk), (v, dv)))
+        g = PosAttnGrads()
+        for t, like, what in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
+            self._rows(t, what, like.shape)
+        d.lse = lse.data_ptr()
+        d.ldo = heads * 64
+        g.dO, g.dQ, g.dK, g.dV = (t.data_ptr() for t in (dout, dq, dk, dv))
+        g.lddo, g.lddq, g.lddk, g.lddv = (self._ld(t, 1, t.shape[2]) for t in (dout, dq, dk, dv))
+        g.bsdo, g.bsdq, g.bsdk, g.bsdv = (self._ld(t, 0, 0) for t in (dout, dq, dk, dv))
+        dtable = torch.empty(d.num_buckets, heads, dtype=torch.float32, device=self.torch_device) if bias is not None else None
+        g.dbias_table = dtable.data_ptr() if dtable is not None else None
+        ws = self._pos_workspace(d, True)
+        self._check(self.lib.pos_attn_bwd(self.h, ctypes.byref(d), ctypes.byref(g)), "pos_attn_bwd")
+        del ws
+        return dq, dk, dv, dtable
 
     def concat_add(self, a, b, c=None):
         rows, C1 = a.shape
