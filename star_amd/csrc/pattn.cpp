@@ -14,7 +14,7 @@ static bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 constexpr int PA_COMP_SPAN = 512;         // rows that see at most this many keys: P and dS with what their rounding left (COMP)
 
-struct PPlan { int gp, rows, units, qb, nw, nq, nblk, nsplit, comp; };
+struct PPlan { int gp, rows, units, qb, nw, nq, nblk, nsplit, per, comp; };
 // the dK / dV pass: units (sequence, K / V head), key blocks, how many of them hold first tokens, in how many parts each kind, slots per unit
 struct PKPlan { int units, nblk, sblk, split_s, split_n, slots; size_t part_slots; };
 
@@ -40,15 +40,21 @@ static PPlan pa_plan(Ctx* ctx, const PAttnArgs& a, bool backward) {
   q.qb = 32 * q.nq * q.nw;
   q.nblk = (q.rows + q.qb - 1) / q.qb;
   if (!backward) {
-    long long span = left + right + 1 + q.qb / q.gp;
-    if (span > a.Nk) span = a.Nk;
-    const long long sinks = a.sinks < a.Nk - span ? a.sinks : a.Nk - span;
-    const long long tiles = (span + 63) / 64 + (sinks + 63) / 64;
+    // the most tiles a block of rows sees: its window, wherever it begins in a tile, and the first tokens
+    const long long all = (a.Nk + 63LL) / 64;
+    long long tiles = (left + right + 2 + q.qb / q.gp + 63) / 64 + 1 + (a.sinks + 63LL) / 64;
+    if (tiles > all) tiles = all;
     const long long base = (long long)q.units * q.nblk, places = (q.nw == 1 ? 5 : 2) * cus;
-    long long s = base > 0 ? places / base : 1;
-    if (s > tiles / 4) s = tiles / 4;
-    if (s > 128) s = 128;
-    q.nsplit = s < 1 ? 1 : (int)s;
+    // tiles per split: the same for all, so that sequences of different lengths make different counts of equal shares
+    long long per = base > 0 ? (tiles * base + places - 1) / places : tiles;
+    if (q.nw == 1) per = (per + 1) / 2;
+    if (per < 4) per = 4;
+    if (per < (tiles + 127) / 128) per = (tiles + 127) / 128;
+    long long s = tiles > 0 ? (tiles + per - 1) / per : 1;
+    if (q.nw != 1 && 2 * base > places) s = 1;
+    if (s < 1) s = 1;
+    q.nsplit = (int)s;
+    q.per = s == 1 ? 0x3fffffff : (int)per;
   }
   return q;
 }
@@ -104,7 +110,7 @@ static PAttnParams pa_params(const PAttnArgs& a, const PPlan& q) {
   p.ldq = a.ldq; p.ldk = a.ldk; p.ldv = a.ldv; p.ldo = a.ldo; p.lddo = a.lddo; p.lddq = a.lddq; p.lddk = a.lddk; p.lddv = a.lddv;
   p.bsq = a.bsq; p.bsk = a.bsk; p.bsv = a.bsv; p.bso = a.bso; p.bsdo = a.bsdo; p.bsdq = a.bsdq; p.bsdk = a.bsdk; p.bsdv = a.bsdv;
   p.Nq = a.Nq; p.Nk = a.Nk; p.heads = a.heads; p.kv_heads = a.kv_heads; p.batch = a.batch;
-  p.gp = q.gp; p.rows = q.rows; p.nblk = q.nblk; p.nsplit = q.nsplit;
+  p.gp = q.gp; p.rows = q.rows; p.nblk = q.nblk; p.nsplit = q.nsplit; p.per = q.per; p.qb = q.qb;
   p.scale = a.scale; p.c = a.scale * PA_LOG2E;
   p.left = a.left < 0 || a.left > PA_NOLIM ? PA_NOLIM : a.left;
   p.right = a.right < 0 || a.right > PA_NOLIM ? PA_NOLIM : a.right;
@@ -144,7 +150,7 @@ size_t pos_attn_workspace(Ctx* ctx, const PAttnArgs& a, bool backward) {
 
 template <class T, int BIAS>
 static int fwd_t(Ctx* ctx, PAttnParams& p, const PPlan& q, dim3 grid) {
-  const size_t smem = 4 * PA_TILE + (BIAS ? (size_t)(2 * p.R + 1) * 4 : 0);
+  const size_t smem = 4 * PA_TILE + (BIAS ? (size_t)(2 * p.R + 1 + 2 * PA_PAD) * 4 : 0);
   if (q.nw == 1) STAR_LAUNCH((pattn_fwd_kernel<T, BIAS, 1, 1, 1>), grid, dim3(64), smem, ctx->stream, p);
   else if (q.comp) STAR_LAUNCH((pattn_fwd_kernel<T, BIAS, 1, 4, 1>), grid, dim3(256), smem, ctx->stream, p);
   else if (q.nq == 1) STAR_LAUNCH((pattn_fwd_kernel<T, BIAS, 1, 4, 0>), grid, dim3(256), smem, ctx->stream, p);
@@ -180,23 +186,23 @@ static int bwd_t(Ctx* ctx, PAttnParams p, const PPlan& q, const PKPlan& kp, floa
   dim3 grid;
   if (p.batch > 0 && p.Nq > 0) {
     if (!pa_grid(p, (long long)q.units * q.nblk, q.units, grid)) return ctx->fail("pos_attn_bwd: too many workgroups");
-    const size_t smem = 4 * PA_TILE + (BIAS ? (size_t)5 * R2 * 4 : 0);
-    STAR_LAUNCH((pattn_dq_kernel<T, BIAS, 1, COMP>), grid, dim3(256), smem, ctx->stream, p);
+    const size_t smem = 4 * PA_TILE + (BIAS ? (size_t)(5 * (R2 + 2 * PA_PAD_Q) + 64 * PA_SKEW + 16) * 4 : 0);
+    STAR_LAUNCH((pattn_dq_kernel<T, BIAS, COMP>), grid, dim3(256), smem, ctx->stream, p);
   }
   if (p.batch > 0 && p.Nk > 0) {
     PAttnParams k = p;
     k.nblk = kp.slots; k.sblk = kp.sblk; k.split_s = kp.split_s; k.split_n = kp.split_n;
     if (!pa_grid(k, (long long)kp.units * kp.slots, kp.units, grid)) return ctx->fail("pos_attn_bwd: too many workgroups");
-    const size_t smem = 2 * (2 * PA_TILE + 64 * 12 + 16) + (BIAS ? (size_t)R2 * 4 : 0);
+    const size_t smem = 2 * (2 * PA_TILE + 64 * 12 + 16) + (BIAS ? (size_t)(R2 + 2 * PA_PAD_K) * 4 : 0);
     STAR_LAUNCH((pattn_dkdv_kernel<T, BIAS, COMP>), grid, dim3(256), smem, ctx->stream, k);
     if (kp.part_slots) {
       const long long blocks = (long long)kp.units * (kp.split_n > 1 ? kp.nblk : kp.sblk);
-      STAR_LAUNCH((pattn_dkdv_join_kernel<T>), dim3((unsigned)blocks), dim3(256), (size_t)0, ctx->stream, k);
+      STAR_LAUNCH((pattn_dkdv_join_kernel<T>), dim3((unsigned)blocks, 8), dim3(256), (size_t)0, ctx->stream, k);
     }
   }
   if (BIAS) {
     PDTableParams t{p.dsum, p.buckets, dtable, p.Nq > 0 ? p.batch : 0, p.heads, q.nblk, p.R, p.num_buckets};
-    STAR_LAUNCH(pattn_dtable_kernel, dim3((unsigned)p.heads), dim3(256), (size_t)R2 * 8, ctx->stream, t);
+    STAR_LAUNCH(pattn_dtable_kernel, dim3((unsigned)p.heads), dim3(256), (size_t)R2 * 8 + (size_t)(R2 + 1) / 2 * 8 + 256 * 8, ctx->stream, t);
   }
   return 0;
 }

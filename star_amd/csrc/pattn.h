@@ -18,8 +18,9 @@
 //     keys once; with a bias a workgroup keeps to one head (one table column in LDS).
 //   * K / V rows that no row of the workgroup sees are staged as zeros through the descriptor's range check: what lies behind kv_len or
 //     outside the window is not read.
-//   * Few rows against long key ranges (a decoding step): the key tiles are dealt to NSPLIT workgroups, each writes its (m, l, O) of the
-//     rows in fp32, pattn_combine_kernel joins them in a fixed order.
+//   * Few rows against long key ranges (a decoding step): the key tiles are dealt to NSPLIT workgroups in equal shares -- sequences of
+//     different lengths make different counts of shares -- each writes its (m, l, O) of the rows in fp32, pattn_combine_kernel joins them
+//     in a fixed order.
 // NQ: 32-row blocks per wave (2: 256-row workgroups for long inputs, 1: 128 rows, more workgroups); NW = 1: a wave by itself, 32 rows.
 // COMP: P is rounded to the 16-bit type, and so is what the rounding left, and both take part in the second product: O is then off by its own
 // rounding alone.  Four more matrix instructions per 32 x 32 block, taken where they do not show: short rows (a few dozen roundings do not
@@ -36,13 +37,13 @@ struct PAttnParams {
   long long bsq, bsk, bsv, bso, bsdo, bsdq, bsdk, bsdv; // batch strides (elements)
   int Nq, Nk, heads, kv_heads, batch;
   int gp;                             // heads packed into one unit's rows (1, or heads / kv_heads)
-  int rows;                           // gp * Nq
+  int rows, qb;                       // gp * Nq; rows per workgroup
   float c, scale;                     // scale * log2(e), scale
   int left, right, sinks;             // left / right past every position: no limit
   const int* q_start; const int* kv_len;
   int start0;                         // position of row 0 where q_start is null
   const float* table; const int* buckets; int num_buckets, R;
-  int nblk, nsplit;                   // row blocks per unit; key splits
+  int nblk, nsplit, per;              // row blocks per unit; key splits, key tiles of each
   long long items;                    // units * nblk * nsplit
   int swz;                            // 1: each XCD walks a contiguous run of items
   float* part;                        // nsplit > 1: [unit][split][rows][68]: O[64], m, l
@@ -94,16 +95,33 @@ STAR_DEV long long pa_item(const PAttnParams& p) {
   return slot >= per ? p.items : (bid & 7) * per + slot;
 }
 
-// the bias of one head by relative position, times log2(e), in LDS: tab[i] belongs to j - p = i - R.  The type's lowest value stays finite
-template <int NT>
+// The bias of one head by relative position, times log2(e), in LDS: tab[i] belongs to j - p = i - R - PAD.  The end values go on for PAD
+// entries either way, so that in a tile that reaches into (-R, R) every score's entry is at a fixed distance from its lane's first: no
+// clamping per score.  The type's lowest value stays finite
+constexpr int PA_PAD = 128, PA_PAD_Q = 96, PA_PAD_K = 192;     // a wave's 64 rows against 64 keys; dQ: 32 rows; dK / dV: 64 rows against 128 keys
+STAR_DEV float pa_bias_at(const PAttnParams& p, int head, int k) {       // of bucket k
+  k = k < 0 ? 0 : k >= p.num_buckets ? p.num_buckets - 1 : k;
+  const float v = p.table[(size_t)k * p.heads + head];
+  const float w = v * PA_LOG2E;
+  return w == PA_NINF && v != PA_NINF ? -3.4028235e38f : w;
+}
+template <int NT, int PAD>
 STAR_DEV void pa_bias_table(const PAttnParams& p, int head, float* tab) {
-  for (int i = threadIdx.x; i < 2 * p.R + 1; i += NT) {
-    int k = p.buckets[i];
-    k = k < 0 ? 0 : k >= p.num_buckets ? p.num_buckets - 1 : k;
-    const float v = p.table[(size_t)k * p.heads + head];
-    float w = v * PA_LOG2E;
-    if (w == PA_NINF && v != PA_NINF) w = -3.4028235e38f;
-    tab[i] = w;
+  constexpr int U = 4;                                 // entries in flight per thread: two dependent loads each
+  const int n = 2 * p.R + 1 + 2 * PAD;
+  for (int i = threadIdx.x; i < n; i += U * NT) {
+    int k[U];
+    float w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      int j = i + u * NT - PAD;
+      j = j < 0 ? 0 : j > 2 * p.R ? 2 * p.R : j;
+      k[u] = p.buckets[j];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = pa_bias_at(p, head, k[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) if (i + u * NT < n) tab[i + u * NT] = w[u];
   }
 }
 
@@ -127,6 +145,25 @@ STAR_DEV PRow pa_row(const PAttnParams& p, int r) {
   if (p.gp == 1) return PRow{r, 0};
   const int i = r / p.gp;
   return PRow{i, r - i * p.gp};
+}
+
+// a wave's rows [r, r + cnt): positions of the first and the last of them, the widest and the narrowest end of their windows.  None: hi = 0
+struct PWave { int p0, p1, hi, lo, hi_min, lo_max; };
+STAR_DEV PWave pa_wave(const PAttnParams& p, const PRange& rg, int r, int cnt) {
+  PWave w;
+  const int last = r + cnt - 1 < p.rows - 1 ? r + cnt - 1 : p.rows - 1;
+  w.p0 = wave_uniform(rg.qs + pa_row(p, r < p.rows ? r : p.rows - 1).i);
+  w.p1 = wave_uniform(rg.qs + pa_row(p, last).i);
+  w.hi = r < p.rows ? pa_hi(p, rg.n, w.p1) : 0;
+  w.lo = pa_lo(p, w.p0);
+  w.hi_min = pa_hi(p, rg.n, w.p0);
+  w.lo_max = pa_lo(p, w.p1);
+  return w;
+}
+// some row sees a key of the tile at k0; every row sees all of its keys
+STAR_DEV bool pa_sees(const PAttnParams& p, const PWave& w, int k0) { return k0 < w.hi && (k0 + PA_KT > w.lo || k0 < p.sinks); }
+STAR_DEV bool pa_sees_whole(const PAttnParams& p, const PWave& w, int k0) {
+  return k0 + PA_KT <= w.hi_min && (k0 >= w.lo_max || k0 + PA_KT <= p.sinks);
 }
 
 // eight rows of d per lane half: acc[db] holds d = 32 db + (r & 3) + 8 (r >> 2) + 4 h2 of the lane's row; 16-byte stores
@@ -181,8 +218,8 @@ pattn_fwd_kernel(const PAttnParams p) {
   const int r_last = r_base + QB - 1 < p.rows - 1 ? r_base + QB - 1 : p.rows - 1;
   const int p0 = wave_uniform(rg.qs + pa_row(p, r_base).i), p1 = wave_uniform(rg.qs + pa_row(p, r_last).i);
   const PTiles tl = pa_tiles(p, n, p0, p1);
-  // a tile is seen whole by every row if it ends before hi_min and begins at lo_max or lies among the first tokens
-  const int hi_min = pa_hi(p, n, p0), lo_max = pa_lo(p, p1);
+  // the wave's own rows: whether they see a tile, see it whole, and how the bias looks there, is asked for them
+  const PWave w = pa_wave(p, rg, r_base + wv * QW, QW);
 
   vec<T, 8> qf[NQ][4];
   int pos[NQ];                                         // position of the lane's row
@@ -196,17 +233,18 @@ pattn_fwd_kernel(const PAttnParams p) {
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) qf[qi][ks] = *reinterpret_cast<const vec<T, 8>*>(q + ks * 16 + h2 * 8);
   }
+  const int total = tl.na + tl.nb;
+  const int it0 = split * p.per < total ? split * p.per : total;
+  const int it1 = split == p.nsplit - 1 || it0 + p.per > total ? total : it0 + p.per;
+  auto tile_of = [&](int it) STAR_ALWAYS_INLINE { return it < tl.na ? it : it - tl.na + tl.b0; };
   float far_l = 0.f, far_r = 0.f;
   if constexpr (BIAS) {
-    pa_bias_table<NT>(p, head0, tab);
+    far_l = pa_bias_at(p, head0, p.buckets[0]); far_r = pa_bias_at(p, head0, p.buckets[2 * p.R]);
+    // where all of the workgroup's tiles are far on the left (most splits of a long cache) only the table's left end is read
+    if (it0 < it1 && tile_of(it1 - 1) * PA_KT + PA_KT - 1 - p0 > -p.R) pa_bias_table<NT, PA_PAD>(p, head0, tab);
+    else for (int i = tid; i <= PA_PAD; i += NT) tab[i] = far_l;
     block_sync();
-    far_l = tab[0]; far_r = tab[2 * p.R];
   }
-
-  const int total = tl.na + tl.nb;
-  const int per = wave_uniform((total + p.nsplit - 1) / p.nsplit);
-  const int it0 = split * per < total ? split * per : total, it1 = it0 + per < total ? it0 + per : total;
-  auto tile_of = [&](int it) STAR_ALWAYS_INLINE { return it < tl.na ? it : it - tl.na + tl.b0; };
   auto stage = [&](int it, int buf) STAR_ALWAYS_INLINE {
     const int t = tile_of(it), k0 = t * PA_KT;
     const int kd = buf * 2 * PA_TILE;
@@ -254,11 +292,12 @@ pattn_fwd_kernel(const PAttnParams p) {
   auto tile = [&](int it, int buf) STAR_ALWAYS_INLINE {
     const int k0 = tile_of(it) * PA_KT;
     const int bofs = buf * 2 * PA_TILE;
-    const bool masked = !(k0 + PA_KT <= hi_min && (k0 >= lo_max || k0 + PA_KT <= p.sinks));
+    if (!pa_sees(p, w, k0)) return;
+    const bool masked = !pa_sees_whole(p, w, k0);
     bool near = false;
     float far = 0.f;
     if constexpr (BIAS) {
-      const bool fl = k0 + PA_KT - 1 - p0 <= -p.R, fr = k0 - p1 >= p.R;
+      const bool fl = k0 + PA_KT - 1 - w.p0 <= -p.R, fr = k0 - w.p1 >= p.R;
       near = !(fl || fr);
       far = fl ? far_l : far_r;
     }
@@ -323,21 +362,17 @@ pattn_fwd_kernel(const PAttnParams p) {
       for (int qi = 0; qi < NQ; ++qi) {
         const int hi = pa_hi(p, n, pos[qi]), lo = pa_lo(p, pos[qi]);
         float mx = PA_NINF;
+        // the table's entry of the lane's first key; a tile past +-R reads the end values that go on there
+        int at = k0 + 4 * h2 - pos[qi];
+        at = at < -p.R - PA_PAD ? -p.R - PA_PAD : at > p.R + PA_PAD - 64 ? p.R + PA_PAD - 64 : at;
+        const float* row = tab + at + p.R + PA_PAD;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int key = k0 + kb * 32 + (r & 3) + 8 * (r >> 2) + 4 * h2;
-            float bias = far;
-            if constexpr (BIAS) {
-              if (near) {
-                int i = key - pos[qi];
-                i = i < -p.R ? -p.R : i > p.R ? p.R : i;
-                bias = tab[i + p.R];
-              }
-            }
-            float y = __builtin_fmaf(s[qi][kb][r], p.c, bias);
-            if (masked && !(key < hi && (key >= lo || key < p.sinks))) y = PA_NINF;
+            const int j = kb * 32 + (r & 3) + 8 * (r >> 2), key = k0 + 4 * h2 + j;
+            float y = __builtin_fmaf(s[qi][kb][r], p.c, BIAS ? row[j] : 0.f);
+            if (masked) y = (key < hi) & ((key >= lo) | (key < p.sinks)) ? y : PA_NINF;
             s[qi][kb][r] = y;
             mx = fmaxf(mx, y);
           }
@@ -376,6 +411,7 @@ pattn_fwd_kernel(const PAttnParams p) {
       }
   };
 
+  if (p.nsplit > 1 && it0 >= it1 && split) return;      // (the first split writes what a row that sees nothing gets)
   glds_wait();                                         // the Q loads are done before the first hand-written LDS-DMA
   if (it0 < it1) stage(it0, 0);
   for (int it = it0; it < it1; ++it) {
@@ -424,17 +460,25 @@ pattn_combine_kernel(const PAttnParams p) {
   const int unit = (int)(row / p.rows), r = (int)(row - (long long)unit * p.rows);
   const float* base = p.part + ((size_t)unit * p.nsplit * p.rows + r) * PA_PART;
   const size_t step = (size_t)p.rows * PA_PART;
+  const PRow rw = pa_row(p, r);
+  const int b = unit / upb;
+  // only the splits that had tiles wrote anything
+  const PRange rg = pa_range(p, b);
+  const int blk = r / p.qb * p.qb, end = blk + p.qb - 1 < p.rows - 1 ? blk + p.qb - 1 : p.rows - 1;
+  const PTiles tl = pa_tiles(p, rg.n, rg.qs + pa_row(p, blk).i, rg.qs + pa_row(p, end).i);
+  const int need = wave_uniform((tl.na + tl.nb + p.per - 1) / p.per), ns = need < 1 ? 1 : need > p.nsplit ? p.nsplit : need;
   float m = PA_NINF;
-  for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, base[s * step + 64]);
+  for (int s = lane; s < ns; s += 64) m = fmaxf(m, base[s * step + 64]);
+  m = wave_max(m);
   float l = 0.f, o = 0.f;
-  for (int s = 0; s < p.nsplit; ++s) {
+#pragma unroll 4
+  for (int s = 0; s < ns; ++s) {
     const float ms = base[s * step + 64];
     const float w = ms == PA_NINF ? 0.f : fast_exp2(ms - m);
     l += w * base[s * step + 65];
     o += w * base[s * step + lane];
   }
-  const PRow rw = pa_row(p, r);
-  const int b = unit / upb, head = (unit - b * upb) * p.gp + rw.g;
+  const int head = (unit - b * upb) * p.gp + rw.g;
   ((T*)p.O)[(size_t)b * p.bso + (size_t)rw.i * p.ldo + head * 64 + lane] = from_f32<T>(l > 0.f ? o / l : l == 0.f ? 0.f : l);
   if (p.lse && lane == 0) p.lse[((size_t)b * p.heads + head) * p.Nq + rw.i] = l == 0.f ? PA_NINF : (m + __builtin_log2f(l)) * PA_LN2;
 }

@@ -43,13 +43,11 @@ STAR_DEV float pa_absmax(const vec<T, 8>* f) {
   return m;
 }
 
-// LDS add of this wave's own array: lanes of one call hit different words, and a wave's LDS operations run in order
-STAR_DEV void lds_add(float* p, float v) {
-#ifdef STAR_HOSTEMU
-  *p += v;
-#else
-  (void)__hip_atomic_fetch_add((__attribute__((address_space(3))) float*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-#endif
+// hi + lo += x, lo gathers what the additions to hi rounded away
+STAR_DEV void pa_add2(float& hi, float& lo, float x) {
+  const float s = hi + x, t = s - hi;
+  lo += (hi - (s - t)) + (x - t);
+  hi = s;
 }
 
 // the rounded value, and what that left
@@ -59,11 +57,14 @@ STAR_DEV void pa_round(float v, T& hi, T& lo) {
   if constexpr (COMP) lo = from_f32<T>(v - to_f32<T>(hi));
 }
 
-template <class T, int BIAS, int NQ, int COMP>
+constexpr int PA_SKEW = 48;                            // floats per row of the skewed buffer: 16 keys + 32 rows - 1 diagonals, and one to spare
+
+// LDS past the tiles with a bias: table | a wave's sums by relative position, four arrays like the table | four skewed buffers
+template <class T, int BIAS, int COMP>
 STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256, 2)
 pattn_dq_kernel(const PAttnParams p) {
-  constexpr int NT = 256, QW = 32 * NQ, QB = 4 * QW;
-  char* smem = dyn_smem();                             // two buffers of (K tile | V tile), bias table, four arrays of sums
+  constexpr int NT = 256, QW = 32, QB = 4 * QW, PAD = PA_PAD_Q;
+  char* smem = dyn_smem();                             // two buffers of (K tile | V tile)
   const long long item = pa_item(p);
   if (item >= p.items) return;
   const int tid = threadIdx.x, lane = tid & 63, wv = wave_uniform(tid >> 6);
@@ -74,9 +75,10 @@ pattn_dq_kernel(const PAttnParams p) {
   const int b = wave_uniform(unit / upb), head0 = wave_uniform((unit - b * upb) * p.gp);
   const int kvh = wave_uniform(head0 / (p.heads / p.kv_heads));
   const PRange rg = pa_range(p, b);
-  const int n = rg.n, R2 = 2 * p.R + 1;
+  const int n = rg.n, RT = 2 * p.R + 1 + 2 * PAD;
   float* tab = reinterpret_cast<float*>(smem + 4 * PA_TILE);
-  float* dsum = tab + (1 + wv) * R2;
+  float* dsum = tab + (1 + wv) * RT;
+  float* skew = tab + 5 * RT + wv * (16 * PA_SKEW);
   const T* Qg = (const T*)p.Q + (size_t)b * p.bsq + head0 * 64;
   const T* Gg = (const T*)p.dO + (size_t)b * p.bsdo + head0 * 64;
   const T* Kg = (const T*)p.K + (size_t)b * p.bsk + kvh * 64;
@@ -86,44 +88,42 @@ pattn_dq_kernel(const PAttnParams p) {
   const int r_last = r_base + QB - 1 < p.rows - 1 ? r_base + QB - 1 : p.rows - 1;
   const int p0 = wave_uniform(rg.qs + pa_row(p, r_base).i), p1 = wave_uniform(rg.qs + pa_row(p, r_last).i);
   const PTiles tl = pa_tiles(p, n, p0, p1);
-  const int hi_min = pa_hi(p, n, p0), lo_max = pa_lo(p, p1);
+  const PWave w = pa_wave(p, rg, r_base + wv * QW, QW);
 
-  vec<T, 8> qf[NQ][4], gf[NQ][4];
-  int pos[NQ], ex[NQ];
-  float lse2[NQ], delta[NQ];
-  bool sole[NQ];                                       // the row sees one key: P = 1
-#pragma unroll
-  for (int qi = 0; qi < NQ; ++qi) {
-    const int r = r_base + wv * QW + qi * 32 + lq;
-    const bool ok = r < p.rows;
-    const PRow rw = pa_row(p, ok ? r : p.rows - 1);
-    pos[qi] = rg.qs + (ok ? rw.i : r);                 // (past the last row: any position, its dS is zero)
+  vec<T, 8> qf[4], gf[4];
+  const int row = r_base + wv * QW + lq;
+  const bool row_ok = row < p.rows;
+  const PRow rw = pa_row(p, row_ok ? row : p.rows - 1);
+  const int pos = rg.qs + (row_ok ? rw.i : row);       // (past the last row: any position, its dS is zero)
+  {
     const T* q = Qg + (size_t)rw.i * p.ldq + rw.g * 64;
     const T* g = Gg + (size_t)rw.i * p.lddo + rw.g * 64;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      qf[qi][ks] = *reinterpret_cast<const vec<T, 8>*>(q + ks * 16 + h2 * 8);
-      gf[qi][ks] = *reinterpret_cast<const vec<T, 8>*>(g + ks * 16 + h2 * 8);
+      qf[ks] = *reinterpret_cast<const vec<T, 8>*>(q + ks * 16 + h2 * 8);
+      gf[ks] = *reinterpret_cast<const vec<T, 8>*>(g + ks * 16 + h2 * 8);
     }
-    const float l = p.lse[((size_t)b * p.heads + head0 + rw.g) * p.Nq + rw.i];
-    lse2[qi] = !ok || l == PA_NINF ? -PA_NINF : l * PA_LOG2E;
-    const int hi = pa_hi(p, n, pos[qi]), lo0 = pa_lo(p, pos[qi]), lo = lo0 < hi ? lo0 : hi;
-    sole[qi] = hi - lo + (p.sinks < lo ? p.sinks : lo) == 1;
-    ex[qi] = 0;
-    if constexpr (__is_same(T, f16)) {
-      const float amax = pair_max(pa_absmax<T>(gf[qi]));
-      ex[qi] = pa_fit_exp(amax);
-      if (ok && h2 == 0) p.st_amax[(size_t)unit * p.rows + r] = amax;
-    }
-    delta[qi] = 0.f;
   }
-  float far_l = 0.f, far_r = 0.f;
-  float sum_l = 0.f, sum_r = 0.f;                      // dS of the keys at -R or before, and at R or past it
+  const float lse_in = p.lse[((size_t)b * p.heads + head0 + rw.g) * p.Nq + rw.i];
+  float lse2 = !row_ok || lse_in == PA_NINF ? -PA_NINF : lse_in * PA_LOG2E;
+  const int hi = pa_hi(p, n, pos), lo0 = pa_lo(p, pos), lo = lo0;
+  const int lo_c = lo0 < hi ? lo0 : hi;
+  const bool sole = hi - lo_c + (p.sinks < lo_c ? p.sinks : lo_c) == 1;        // the row sees one key: P = 1
+  float exf = 0.f, ipw = 1.f;                          // f16: dS is rounded as 2^ex dS; ex and 2^-ex
+  if constexpr (__is_same(T, f16)) {
+    const float amax = pair_max(pa_absmax<T>(gf));
+    const int ex = pa_fit_exp(amax);
+    exf = (float)ex; ipw = pa_pow2(-ex);
+    if (row_ok && h2 == 0) p.st_amax[(size_t)unit * p.rows + row] = amax;
+  }
+  float delta = 0.f, lsum = 0.f, delta_lo = 0.f, lsum_lo = 0.f, far_l = 0.f, far_r = 0.f;
+  float sum_l = 0.f, sum_r = 0.f;                      // dS of far tiles: keys at -R or before, at R or past it; what the adds rounded away
+  float low_l = 0.f, low_r = 0.f;
   if constexpr (BIAS) {
-    pa_bias_table<NT>(p, head0, tab);
-    for (int i = lane; i < R2; i += 64) dsum[i] = 0.f;
+    pa_bias_table<NT, PAD>(p, head0, tab);
+    for (int i = tid; i < 4 * RT + 64 * PA_SKEW; i += NT) tab[RT + i] = 0.f;
     block_sync();
-    far_l = tab[0]; far_r = tab[2 * p.R];
+    far_l = tab[0]; far_r = tab[RT - 1];
   }
 
   const int total = tl.na + tl.nb;
@@ -157,141 +157,124 @@ pattn_dq_kernel(const PAttnParams p) {
         tfo[half][db] = opaque(smem + swz_off(key, d >> 3) + (d & 7) * 2);
       }
   }
-  f32x16 acc[NQ][2];
+  f32x16 acc[2];
 #pragma unroll
-  for (int a = 0; a < NQ; ++a)
+  for (int c2 = 0; c2 < 2; ++c2)
 #pragma unroll
-    for (int c2 = 0; c2 < 2; ++c2)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[a][c2][r] = 0.f;
-  float lsum[NQ];
-#pragma unroll
-  for (int qi = 0; qi < NQ; ++qi) lsum[qi] = 0.f;
+    for (int r = 0; r < 16; ++r) acc[c2][r] = 0.f;
+  float lse_x = lse2;                                  // subtracted from the exponent: second walk less ex
 
-  // one tile of 64 keys; WALK 0: delta and the row sum, WALK 1: dS and dQ
-  auto tile = [&](int it, int buf, auto walk_tag) STAR_ALWAYS_INLINE {
-    constexpr int WALK = decltype(walk_tag)::value;
-    const int k0 = tile_of(it) * PA_KT;
-    const int bofs = buf * 2 * PA_TILE;
-    const bool masked = !(k0 + PA_KT <= hi_min && (k0 >= lo_max || k0 + PA_KT <= p.sinks));
-    bool near = false, fl = false;
-    float far = 0.f;
-    if constexpr (BIAS) {
-      fl = k0 + PA_KT - 1 - p0 <= -p.R;
-      near = !(fl || k0 - p1 >= p.R);
-      far = fl ? far_l : far_r;
-    }
+  // one tile of 64 keys.  WALK 0: delta and the row sum, WALK 1: dS and dQ.  KIND 0: every row sees every key, the bias is one constant;
+  // 1: masks; 2: masks, the bias from the table, dS into the sums by relative position.  KIND 0: both halves' products come first, the second
+  // half's run beside the first half's vector work (the other kinds have no registers left for that)
+  auto body = [&](int k0, int bofs, bool masked, bool fl, float far, vec<T, 8>* ds, vec<T, 8>* dr, auto walk_tag, auto kind_tag) STAR_ALWAYS_INLINE {
+    constexpr int WALK = decltype(walk_tag)::value, KIND = decltype(kind_tag)::value;
+    constexpr bool AHEAD = KIND == 0 && !COMP;
+    f32x16 s[2], dp[2];
+    auto products = [&](int kb) STAR_ALWAYS_INLINE {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      f32x16 s[NQ], dp[NQ];
-#pragma unroll
-      for (int qi = 0; qi < NQ; ++qi)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) { s[qi][r] = 0.f; dp[qi][r] = 0.f; }
+      for (int r = 0; r < 16; ++r) { s[kb][r] = 0.f; dp[kb][r] = 0.f; }
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         const vec<T, 8> kf = *reinterpret_cast<const vec<T, 8>*>(kfo[ks] + bofs + kb * 4096);
         const vec<T, 8> vf = *reinterpret_cast<const vec<T, 8>*>(kfo[ks] + bofs + PA_TILE + kb * 4096);
-#pragma unroll
-        for (int qi = 0; qi < NQ; ++qi) {
-          s[qi] = mfma32<T>(kf, qf[qi][ks], s[qi]);
-          dp[qi] = mfma32<T>(vf, gf[qi][ks], dp[qi]);
-        }
+        s[kb] = mfma32<T>(kf, qf[ks], s[kb]);
+        dp[kb] = mfma32<T>(vf, gf[ks], dp[kb]);
       }
-      vec<T, 8> ds[NQ][2], dl8[COMP ? NQ : 1][2];
-      // WALK 1: the rounded dS' = 2^ex dS of score r, and dS into the sums by relative position (far tiles: one sum)
-      if (!masked && !near) {
+    };
+    if constexpr (AHEAD) { products(0); products(1); }
+    const float off = far - lse_x;
+    float t0 = 0.f, t1 = 0.f, l0 = 0.f, l1 = 0.f;        // this tile's sums
 #pragma unroll
-        for (int qi = 0; qi < NQ; ++qi) {
-          const float off = far - lse2[qi];
-          if constexpr (WALK == 0) {
-            float a0 = 0.f, a1 = 0.f, d0 = 0.f, d1 = 0.f;
+    for (int kb = 0; kb < 2; ++kb) {
+      if constexpr (!AHEAD) { STAR_SCHED_FENCE(); products(kb); }
+      const int at = k0 + kb * 32 + 4 * h2 - pos + p.R + PAD;                  // the table's entry of the lane's first key
 #pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-              const float pa = fast_exp2(__builtin_fmaf(s[qi][r], p.c, off)), pb = fast_exp2(__builtin_fmaf(s[qi][r + 1], p.c, off));
-              a0 += pa; a1 += pb;
-              d0 = __builtin_fmaf(pa, dp[qi][r], d0); d1 = __builtin_fmaf(pb, dp[qi][r + 1], d1);
-            }
-            lsum[qi] += a0 + a1; delta[qi] += d0 + d1;
-          } else {
-            const float pw = pa_pow2(ex[qi]), dl = -delta[qi] * pw;
-            float t0 = 0.f, t1 = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float v = fast_exp2(__builtin_fmaf(s[qi][r], p.c, off)) * __builtin_fmaf(dp[qi][r], pw, dl);
-              if constexpr (BIAS) { if (r & 1) t1 += v; else t0 += v; }
-              T hi16, lo16{};
-              pa_round<T, COMP>(v, hi16, lo16);
-              ds[qi][r >> 3][r & 7] = hi16;
-              if constexpr (COMP) dl8[qi][r >> 3][r & 7] = lo16;
-            }
-            if constexpr (BIAS) {
-              const float t = (t0 + t1) * pa_pow2(-ex[qi]);
-              sum_l += fl ? t : 0.f;
-              sum_r += fl ? 0.f : t;
-            }
-          }
+      for (int r = 0; r < 16; ++r) {
+        const int j = (r & 3) + 8 * (r >> 2), key = k0 + kb * 32 + j + 4 * h2;
+        float x = __builtin_fmaf(s[kb][r], p.c, KIND == 2 ? tab[at + j] - lse_x : off);
+        bool see = true;
+        if constexpr (KIND != 0) {
+          see = !masked | ((key < hi) & ((key >= lo) | (key < p.sinks)));
+          x = sole ? (WALK ? exf : 0.f) : x;
         }
-      } else {
+        float pr = fast_exp2(x);
+        if constexpr (KIND != 0) pr = see ? pr : 0.f;
+        if constexpr (WALK == 0) {
+          const float d = KIND != 0 ? (see ? dp[kb][r] : 0.f) : dp[kb][r];
+          if (r & 1) { l1 += pr; t1 = __builtin_fmaf(pr, d, t1); }
+          else { l0 += pr; t0 = __builtin_fmaf(pr, d, t0); }
+        } else {
+          // (subtracted at the end: a row with one visible key has dP - delta = 0 exactly, and sums that start at -delta cost the table's
+          // gradient half of its digits past 1e-6)
+          float v = pr * (dp[kb][r] - delta);
+          if constexpr (KIND != 0) v = see ? v : 0.f;
+          T hi16, lo16{};
+          pa_round<T, COMP>(v, hi16, lo16);
+          ds[2 * kb + (r >> 3)][r & 7] = hi16;
+          if constexpr (COMP) dr[2 * kb + (r >> 3)][r & 7] = lo16;
+          if constexpr (BIAS && KIND != 2) { if (r & 1) t1 += v; else t0 += v; }
+          if constexpr (KIND == 2) {
+            // sums along the diagonals, sixteen keys at a time: each row of values is stored one word further on, so that a relative
+            // position becomes a column (the other cells of a row stay zero), and a lane adds up a column.  The rows' positions go
+            // up by one lane by lane: with a bias a unit is one head
+            skew[((j & 15) + 4 * h2) * (PA_SKEW + 1) - lq + 31] = v * ipw;
+            if ((r & 7) == 7) {
+              wave_lds_order();
+              if (lane < PA_SKEW - 1) {
+                float c0 = 0.f, c1 = 0.f;
 #pragma unroll
-        for (int qi = 0; qi < NQ; ++qi) {
-          const int hi = pa_hi(p, n, pos[qi]), lo = pa_lo(p, pos[qi]);
-          const float pw = pa_pow2(ex[qi]), ipw = pa_pow2(-ex[qi]), dl = -delta[qi] * pw;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = k0 + kb * 32 + (r & 3) + 8 * (r >> 2) + 4 * h2;
-            const int rel = key - pos[qi];
-            float bias = far;
-            if constexpr (BIAS) {
-              if (near) { const int i = rel < -p.R ? -p.R : rel > p.R ? p.R : rel; bias = tab[i + p.R]; }
-            }
-            float x = __builtin_fmaf(s[qi][r], p.c, bias - lse2[qi]);
-            if (sole[qi]) x = 0.f;
-            const bool see = !masked || (key < hi && (key >= lo || key < p.sinks));
-            const float pr = see ? fast_exp2(x) : 0.f;
-            if constexpr (WALK == 0) {
-              lsum[qi] += pr;
-              delta[qi] += see ? pr * dp[qi][r] : 0.f;
-            } else {
-              const float v = see ? pr * __builtin_fmaf(dp[qi][r], pw, dl) : 0.f;
-              T hi16, lo16{};
-              pa_round<T, COMP>(v, hi16, lo16);
-              ds[qi][r >> 3][r & 7] = hi16;
-              if constexpr (COMP) dl8[qi][r >> 3][r & 7] = lo16;
-              if constexpr (BIAS) {
-                const float w = v * ipw;
-                sum_l += rel <= -p.R ? w : 0.f;
-                sum_r += rel > -p.R && rel >= p.R ? w : 0.f;
-                // the lanes of one half hold different rows of one key: their words differ; the halves go one after the other
-#pragma unroll
-                for (int hh = 0; hh < 2; ++hh) {
-                  if (h2 == hh && rel > -p.R && rel < p.R) lds_add(dsum + rel + p.R, w);
-                  wave_lds_order();
-                }
+                for (int i = 0; i < 16; i += 2) { c0 += skew[i * PA_SKEW + lane]; c1 += skew[(i + 1) * PA_SKEW + lane]; }
+                float* to = dsum + (k0 + kb * 32 + 16 * (r >> 3) - (w.p0 + 31) + p.R + PAD) + lane;
+                *to += c0 + c1;
               }
+              wave_lds_order();
             }
           }
         }
       }
-      if constexpr (WALK == 1) {
+    }
+    if constexpr (WALK == 0) {
+      // (with a bias to 2^-48: what delta is off by stays in the sums over millions of pairs that make up the table's gradient)
+      if constexpr (BIAS) { pa_add2(lsum, lsum_lo, l0 + l1); pa_add2(delta, delta_lo, t0 + t1); }
+      else { lsum += l0 + l1; delta += t0 + t1; }
+    }
+    else if constexpr (BIAS && KIND != 2) {
+      const float t = (t0 + t1) * ipw;
+      pa_add2(sum_l, low_l, fl ? t : 0.f);
+      pa_add2(sum_r, low_r, fl ? 0.f : t);
+    }
+  };
+  auto tile = [&](int it, int buf, auto walk_tag) STAR_ALWAYS_INLINE {
+    const int k0 = tile_of(it) * PA_KT, bofs = buf * 2 * PA_TILE;
+    if (!pa_sees(p, w, k0)) return;
+    const bool masked = !pa_sees_whole(p, w, k0);
+    bool near = false, fl = false;
+    float far = 0.f;
+    if constexpr (BIAS) {
+      fl = k0 + PA_KT - 1 - w.p0 <= -p.R;
+      near = !(fl || k0 - w.p1 >= p.R);
+      far = fl ? far_l : far_r;
+    }
+    vec<T, 8> ds[4], dr[4];                            // 2^ex dS, sixteen keys each, and what its rounding left
+    if (BIAS && near) body(k0, bofs, masked, fl, far, ds, dr, walk_tag, std::integral_constant<int, BIAS ? 2 : 1>{});
+    else if (masked) body(k0, bofs, masked, fl, far, ds, dr, walk_tag, std::integral_constant<int, 1>{});
+    else body(k0, bofs, masked, fl, far, ds, dr, walk_tag, std::integral_constant<int, 0>{});
+    if constexpr (decltype(walk_tag)::value == 1) {    // (outside the kinds: accumulators that they all write are copied from one to the other)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int db = 0; db < 2; ++db) {
-            vec<T, 8> kt;
+        for (int db = 0; db < 2; ++db) {
+          vec<T, 8> kt;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const vec<T, 4> r = lds_read_tr<T>(tfo[half][db] + bofs + (kb * 2 + u) * 2048);
+          for (int half = 0; half < 2; ++half) {
+            const vec<T, 4> r = lds_read_tr<T>(tfo[half][db] + bofs + u * 2048);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) kt[half * 4 + e] = r[e];
-            }
-#pragma unroll
-            for (int qi = 0; qi < NQ; ++qi) {
-              acc[qi][db] = mfma32<T>(kt, ds[qi][u], acc[qi][db]);
-              if constexpr (COMP) acc[qi][db] = mfma32<T>(kt, dl8[qi][u], acc[qi][db]);
-            }
+            for (int e = 0; e < 4; ++e) kt[half * 4 + e] = r[e];
           }
-      }
+          acc[db] = mfma32<T>(kt, ds[u], acc[db]);
+          if constexpr (COMP) acc[db] = mfma32<T>(kt, dr[u], acc[db]);
+        }
     }
   };
 
@@ -303,16 +286,15 @@ pattn_dq_kernel(const PAttnParams p) {
     stage(it + 1 < total ? it + 1 : 0, buf ^ 1);       // (the second walk's first tile behind the last)
     tile(it, buf, std::integral_constant<int, 0>{});
   }
-#pragma unroll
-  for (int qi = 0; qi < NQ; ++qi) {
-    const float l = pair_sum(lsum[qi]), d = pair_sum(delta[qi]);
-    delta[qi] = l > 0.f ? d / l : l == 0.f ? 0.f : l;
-    if (l > 0.f) lse2[qi] += __builtin_log2f(l);
-    const int r = r_base + wv * QW + qi * 32 + lq;
-    if (r < p.rows && h2 == 0) {
-      const size_t at = (size_t)unit * p.rows + r;
-      p.st_lse[at] = lse2[qi];
-      p.st_delta[at] = delta[qi];
+  {
+    const float l = pair_sum(lsum + lsum_lo), d = pair_sum(delta + delta_lo);
+    delta = l > 0.f ? d / l : l == 0.f ? 0.f : l;
+    if (l > 0.f) lse2 += __builtin_log2f(l);
+    lse_x = lse2 - exf;
+    if (row_ok && h2 == 0) {
+      const size_t at = (size_t)unit * p.rows + row;
+      p.st_lse[at] = lse2;
+      p.st_delta[at] = delta;
     }
   }
   for (int it = 0; it < total; ++it, buf ^= 1) {
@@ -320,22 +302,29 @@ pattn_dq_kernel(const PAttnParams p) {
     if (it + 1 < total) stage(it + 1, buf ^ 1);
     tile(it, buf, std::integral_constant<int, 1>{});
   }
-#pragma unroll
-  for (int qi = 0; qi < NQ; ++qi) {
-    const int r = r_base + wv * QW + qi * 32 + lq;
-    const bool ok = r < p.rows;
-    const PRow rw = pa_row(p, ok ? r : p.rows - 1);
-    pa_store_row<T>(acc[qi], p.scale * pa_pow2(-ex[qi]), (T*)p.dQ + (size_t)b * p.bsdq + (size_t)rw.i * p.lddq + (head0 + rw.g) * 64, ok);
-  }
+  pa_store_row<T>(acc, p.scale * ipw, (T*)p.dQ + (size_t)b * p.bsdq + (size_t)rw.i * p.lddq + (head0 + rw.g) * 64, row_ok);
   if constexpr (BIAS) {
-    const float tl2 = wave_sum(sum_l), tr2 = wave_sum(sum_r);
-    if (lane == 0) {
-      if (p.R > 0) { dsum[0] = tl2; dsum[2 * p.R] = tr2; }
-      else dsum[0] = tl2 + tr2;
-    }
+    const float tl2 = wave_sum(sum_l + low_l), tr2 = wave_sum(sum_r + low_r);
+    block_sync();                                      // every wave is past its last read of a tile: the buffers' first words are free
+    float* ends = reinterpret_cast<float*>(smem);
+    if (lane == 0) { ends[wv] = tl2; ends[4 + wv] = tr2; }
     block_sync();
+    // entry i of the arrays belongs to j - p = i - R - PAD; what lies at +-R and past it joins the far tiles' sums
+    auto column = [&](int i) { return (tab[RT + i] + tab[2 * RT + i]) + (tab[3 * RT + i] + tab[4 * RT + i]); };
+    const int R2 = 2 * p.R + 1;
     float* out = p.dsum + ((size_t)unit * p.nblk + qb) * R2;
-    for (int i = tid; i < R2; i += NT) out[i] = (tab[R2 + i] + tab[2 * R2 + i]) + (tab[3 * R2 + i] + tab[4 * R2 + i]);
+    for (int i = 1 + tid; i < R2 - 1; i += NT) out[i] = column(i + PAD);
+    float e = 0.f;                                     // first wave: the columns up to -R; last wave: from R on (R = 0: past it)
+    if (wv == 0) for (int i = lane; i <= PAD; i += 64) e += column(i);
+    if (wv == 3) for (int i = lane; i <= PAD - (p.R == 0); i += 64) e += column(RT - 1 - i);
+    e = wave_sum(e);
+    if (lane == 0) ends[8 + wv] = e;
+    block_sync();
+    if (tid == 0) {
+      const float left = ends[8] + ((ends[0] + ends[1]) + (ends[2] + ends[3])), right = ends[11] + ((ends[4] + ends[5]) + (ends[6] + ends[7]));
+      if (p.R > 0) { out[0] = left; out[R2 - 1] = right; }
+      else out[0] = left + right;
+    }
   }
 }
 
@@ -353,7 +342,7 @@ STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256, 2)
 pattn_dkdv_kernel(const PAttnParams p) {
   constexpr int NT = 256, KB = 128, QT = 64;           // keys per workgroup, query rows per tile
   constexpr int SHIFT = __is_same(T, f16) ? 10 : 0;    // P is rounded as 2^SHIFT P
-  constexpr int ROWB = QT * 12 + 16, BUF = 2 * PA_TILE + ROWB;   // Q tile | dO tile | off[64] | delta[64] | pos[64] | exponent
+  constexpr int ROWB = QT * 12 + 16, BUF = 2 * PA_TILE + ROWB;   // Q tile | dO tile | off[64] | -delta[64] | pos[64] | exponent
   char* smem = dyn_smem();                             // two such buffers, then the bias table
   const long long item = pa_item(p);
   if (item >= p.items) return;
@@ -446,9 +435,9 @@ pattn_dkdv_kernel(const PAttnParams p) {
     float far_l = 0.f, far_r = 0.f;
     if constexpr (BIAS) {
       block_sync();                                    // the last tile's readers are done with the table
-      pa_bias_table<NT>(p, head0, tab);
+      pa_bias_table<NT, PA_PAD_K>(p, head0, tab);
       block_sync();
-      far_l = tab[0]; far_r = tab[2 * p.R];
+      far_l = tab[0]; far_r = tab[2 * p.R + 2 * PA_PAD_K];
     } else block_sync();
 
     auto bounds = [&](int t, int& pa, int& pb) STAR_ALWAYS_INLINE {    // positions of a tile's first and last row
@@ -494,7 +483,7 @@ pattn_dkdv_kernel(const PAttnParams p) {
         if (m > 0.f) { const int e = pa_fit_exp(m); if (e < e_row) e_row = e; }
       }
       o[tid] = far - x_lse + (float)SHIFT;
-      o[64 + tid] = SHIFT ? x_delta * pa_pow2(e_row - SHIFT) : x_delta;
+      o[64 + tid] = -x_delta;
       reinterpret_cast<int*>(o)[128 + tid] = rg.qs + pa_row(p, t * QT + tid).i;
       if (SHIFT && tid == 0) reinterpret_cast<int*>(o)[192] = e_row;
     };
@@ -521,11 +510,20 @@ pattn_dkdv_kernel(const PAttnParams p) {
       if (jw >= n || jw > pb + p.right || (jl < pa - p.left && jw >= p.sinks)) return;   // no row of the tile sees a key of the wave
       const bool masked = !(jl < n && jl <= pa + p.right && (jw >= pb - p.left || jl < p.sinks));
       const bool near = BIAS ? !(j0 + KB - 1 - pa <= -p.R || j0 - pb >= p.R) : false;
+      const bool table = BIAS && near, plain = !table && !masked;
 #pragma unroll
       for (int qs = 0; qs < 2; ++qs) {
         f32x16 s, dp;
 #pragma unroll
         for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+        if (plain) {                                     // the sums of dP start at -delta (else it is added at the end, as in dQ)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4 dl = *reinterpret_cast<const f32x4*>(o + 64 + qs * 32 + 8 * g + 4 * h2);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dp[4 * g + e] = dl[e];
+          }
+        }
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           const vec<T, 8> a = *reinterpret_cast<const vec<T, 8>*>(afo[ks] + bofs + qs * 4096);
@@ -533,34 +531,36 @@ pattn_dkdv_kernel(const PAttnParams p) {
           s = mfma32<T>(a, kf[ks], s);
           dp = mfma32<T>(g, vf[ks], dp);
         }
-        vec<T, 8> pf[2], df[2], pl[2], dl8[2];
+        vec<T, 8> pf[2], df[2], pl[2], dl8[2];           // P and dS, sixteen rows each, and what their rounding left
+        // KIND 0: every row sees every key, the bias is one constant (in off); 1: masks; 2: masks, and the bias from the table
+        auto weights = [&](auto kind_tag) STAR_ALWAYS_INLINE {
+          constexpr int KIND = decltype(kind_tag)::value;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {                    // rows 8 g + 4 h2 + (0 .. 3) of the 32
-          const int row = qs * 32 + 8 * g + 4 * h2;
-          const f32x4 off = *reinterpret_cast<const f32x4*>(o + row), dl = *reinterpret_cast<const f32x4*>(o + 64 + row);
-          if (!masked && !near) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float pr = fast_exp2(__builtin_fmaf(s[4 * g + e], p.c, off[e]));
-              const float v = pr * (SHIFT ? __builtin_fmaf(dp[4 * g + e], pw, -dl[e]) : dp[4 * g + e] - dl[e]);
-              T a, al{}, d, dl_{};
-              pa_round<T, COMP>(pr, a, al);
-              pa_round<T, COMP>(v, d, dl_);
-              pf[g >> 1][(g & 1) * 4 + e] = a; df[g >> 1][(g & 1) * 4 + e] = d;
-              if constexpr (COMP) { pl[g >> 1][(g & 1) * 4 + e] = al; dl8[g >> 1][(g & 1) * 4 + e] = dl_; }
+          for (int g = 0; g < 4; ++g) {                  // rows 8 g + 4 h2 + (0 .. 3) of the 32
+            const int row = qs * 32 + 8 * g + 4 * h2;
+            const f32x4 off = *reinterpret_cast<const f32x4*>(o + row);
+            vec<int, 4> ps{};
+            f32x4 dl{};
+            if constexpr (KIND != 0) {
+              dl = *reinterpret_cast<const f32x4*>(o + 64 + row);
+              ps = *reinterpret_cast<const vec<int, 4>*>(reinterpret_cast<const int*>(o) + 128 + row);
             }
-          } else {
-            const vec<int, 4> ps = *reinterpret_cast<const vec<int, 4>*>(reinterpret_cast<const int*>(o) + 128 + row);
+            // (with a bias a unit is one head: row by row the positions go up by one)
+            const float* tb = KIND == 2 ? tab + (key - (rg.qs + t * QT + row + 3) + p.R + PA_PAD_K) : nullptr;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int rel = key - ps[e];
-              float of = off[e];
-              if constexpr (BIAS) {
-                if (near) { const int i = rel < -p.R ? -p.R : rel > p.R ? p.R : rel; of += tab[i + p.R]; }
+              const int r = 4 * g + e;
+              float add = off[e];
+              if constexpr (KIND == 2) add += tb[3 - e];
+              float pr = fast_exp2(__builtin_fmaf(s[r], p.c, add));
+              const float d0 = KIND == 0 ? dp[r] : dp[r] + dl[e];
+              float v = pr * (SHIFT ? d0 * pw : d0);
+              if constexpr (KIND != 0) {
+                const int rel = key - ps[e];
+                const bool see = !masked | ((key < n) & (rel <= p.right) & ((rel >= -p.left) | (key < p.sinks)));
+                pr = see ? pr : 0.f;
+                v = see ? v : 0.f;
               }
-              const bool see = !masked || (key < n && rel <= p.right && (rel >= -p.left || key < p.sinks));
-              const float pr = see ? fast_exp2(__builtin_fmaf(s[4 * g + e], p.c, of)) : 0.f;
-              const float v = see ? pr * (SHIFT ? __builtin_fmaf(dp[4 * g + e], pw, -dl[e]) : dp[4 * g + e] - dl[e]) : 0.f;
               T a, al{}, d, dl_{};
               pa_round<T, COMP>(pr, a, al);
               pa_round<T, COMP>(v, d, dl_);
@@ -568,7 +568,10 @@ pattn_dkdv_kernel(const PAttnParams p) {
               if constexpr (COMP) { pl[g >> 1][(g & 1) * 4 + e] = al; dl8[g >> 1][(g & 1) * 4 + e] = dl_; }
             }
           }
-        }
+        };
+        if (table) weights(std::integral_constant<int, BIAS ? 2 : 1>{});
+        else if (masked) weights(std::integral_constant<int, 1>{});
+        else weights(std::integral_constant<int, 0>{});
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -626,7 +629,7 @@ pattn_dkdv_kernel(const PAttnParams p) {
   pa_store_row<T>(dv, mv, (T*)p.dV + (size_t)ob * p.bsdv + (size_t)(ok ? key : 0) * p.lddv + kvh * 64, ok);
 }
 
-// adds the parts of the key blocks that were split, in their order: one workgroup per block, a thread per eight values
+// adds the parts of the key blocks that were split, in their order: eight workgroups per block, a thread per eight values
 template <class T>
 STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256)
 pattn_dkdv_join_kernel(const PAttnParams p) {
@@ -638,7 +641,7 @@ pattn_dkdv_join_kernel(const PAttnParams p) {
   const int per = p.split_n > 1 ? p.nblk : first;
   const int b = ku / p.kv_heads, kvh = ku - b * p.kv_heads;
   const float* src = p.part + ((size_t)ku * per + slot) * 128 * 128;
-  for (int i = threadIdx.x; i < 128 * 16; i += 256) {
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < 128 * 16; i += 256 * gridDim.y) {
     const int row = i >> 4, c = (i & 15) * 8, key = k * 128 + row;
     if (key >= p.Nk) continue;
     float v[8];
@@ -661,9 +664,12 @@ pattn_dkdv_join_kernel(const PAttnParams p) {
 struct PDTableParams { const float* dsum; const int* buckets; float* dtable; int batch, heads, nblk, R, num_buckets; };
 STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256)
 pattn_dtable_kernel(const PDTableParams p) {
-  double* rel = reinterpret_cast<double*>(dyn_smem());
   const int h = blockIdx.x, R2 = 2 * p.R + 1;
+  double* rel = reinterpret_cast<double*>(dyn_smem());
+  int* of = reinterpret_cast<int*>(rel + R2);
   for (int i = threadIdx.x; i < R2; i += 256) {
+    const int c = p.buckets[i];
+    of[i] = c < 0 ? 0 : c >= p.num_buckets ? p.num_buckets - 1 : c;
     double s = 0.0;
     for (int b = 0; b < p.batch; ++b) {
       const float* d = p.dsum + ((size_t)b * p.heads + h) * p.nblk * R2 + i;
@@ -673,14 +679,23 @@ pattn_dtable_kernel(const PDTableParams p) {
     rel[i] = s;
   }
   block_sync();
-  for (int k = threadIdx.x; k < p.num_buckets; k += 256) {
+  // a bucket's entries are shared out among `slices` threads, joined in a fixed order
+  int nb = 1;
+  while (nb < p.num_buckets && nb < 256) nb <<= 1;
+  const int slices = 256 / nb, me = threadIdx.x / nb;
+  double* part = rel + R2 + (R2 + 1) / 2;              // [256], past the bucket numbers
+  for (int k0 = 0; k0 < p.num_buckets; k0 += nb) {
+    const int k = k0 + (int)threadIdx.x % nb;
     double s = 0.0;
-    for (int i = 0; i < R2; ++i) {
-      int c = p.buckets[i];
-      c = c < 0 ? 0 : c >= p.num_buckets ? p.num_buckets - 1 : c;
-      if (c == k) s += rel[i];
+#pragma unroll 4
+    for (int i = me; i < R2; i += slices) { const double v = rel[i]; s += of[i] == k ? v : 0.0; }
+    part[threadIdx.x] = s;
+    block_sync();
+    if (me == 0 && k < p.num_buckets) {
+      for (int q = 1; q < slices; ++q) s += part[q * nb + threadIdx.x];
+      p.dtable[(size_t)k * p.heads + h] = (float)s;
     }
-    p.dtable[(size_t)k * p.heads + h] = (float)s;
+    block_sync();
   }
 }
 

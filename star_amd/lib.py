@@ -189,6 +189,10 @@ def _ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
 
 
+# the current stream's handle without the Python object around it (1.1 us of a 9 us call), where torch has such a thing
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _addr(t):
     return None if t is None else t.data_ptr()
 
@@ -229,8 +233,8 @@ class Context:
                    6: "the device is not a gfx950 (MI355X) with the 160 KB LDS opt-in"}.get(rc, "")
             raise StarError(f"star_ctx_create failed (rc={rc}) {why}")
         self.h = h
-        if not self.lib.is_hostemu:
-            self.lib.set_stream(self.h, ctypes.c_void_p(torch.cuda.current_stream(self.device_index).cuda_stream))
+        self._stream = None             # what star_set_stream was last told
+        self.use_current_stream()
 
     def trim(self):
         """give the arena's cached blocks back to the driver (phase boundaries; the reference calls torch.cuda.empty_cache() there)"""
@@ -265,7 +269,8 @@ class Context:
 
     def use_current_stream(self):
         if not self.lib.is_hostemu:
-            self.lib.set_stream(self.h, ctypes.c_void_p(torch.cuda.current_stream(self.device_index).cuda_stream))
+            s = torch.cuda.current_stream(self.device_index).cuda_stream
+            self._stream = s if self.lib.set_stream(self.h, ctypes.c_void_p(s)) == 0 else None
 
     def profile_begin(self, kinds=None):
         """HIP events around every launch, or only around the families named in `kinds` (PROF_KINDS names): events cost stream time"""
@@ -476,34 +481,40 @@ class Context:
     # These calls follow torch's current stream, allocate what they return and their workspaces there, and leave the arena alone: they may
     # be captured into graphs, and calls on several streams do not share scratch memory.
     def _rows(self, t, what, shape=None, dtype=None):
-        """rows of a [..., C] tensor with unit column stride: checked, and with a stride that says something where there is one row"""
+        """a [..., C] tensor of the context's device and type with unit column stride"""
         if not isinstance(t, torch.Tensor):
             raise StarError(f"{what} must be a tensor")
-        self._chk_tensor(t, dtype or self.dtype)
-        if shape is not None and tuple(t.shape) != tuple(shape):
+        if t.dtype is not (dtype or self.dtype) or t.device != self.torch_device:
+            self._chk_tensor(t, dtype or self.dtype)
+        if shape is not None and t.shape != shape:
             raise StarError(f"{what} must be {list(shape)}, got {list(t.shape)}")
-        if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        if t.stride(-1) != 1 and t.numel() and t.shape[-1] > 1:
             raise StarError(f"{what} must have unit stride in its last dimension")
-        return t
 
     def _vec_f32(self, t, n, what):
         if t is None:
             return
-        self._chk_tensor(t, torch.float32)
-        if tuple(t.shape) != (n,) or not t.is_contiguous():
+        if t.dtype is not torch.float32 or t.device != self.torch_device:
+            self._chk_tensor(t, torch.float32)
+        if t.shape != (n,) or not t.is_contiguous():
             raise StarError(f"{what} must be a contiguous fp32 [{n}]")
 
     @staticmethod
     def _ld(t, dim, width):
         """stride of `dim`; a dimension of one row has whatever stride torch left there"""
         ld = t.stride(dim) if t.shape[dim] > 1 and t.numel() else width
-        if dim == t.dim() - 2 and ld >= 2 ** 31:
+        if ld >= 2 ** 31 and dim:
             raise StarError(f"a row stride of {ld} elements is too large")
         return ld
 
     def _follow_stream(self):
-        if not self.lib.is_hostemu:
-            self._check(self.lib.set_stream(self.h, torch.cuda.current_stream(self.device_index).cuda_stream), "set_stream")
+        """torch's current stream on this device becomes the context's (a call of its own only where it changed)"""
+        if self.lib.is_hostemu:
+            return
+        s = _raw_stream(self.device_index)
+        if s != self._stream:
+            self._check(self.lib.set_stream(self.h, s), "set_stream")
+            self._stream = s
 
     def layer_norm_train(self, x, gamma=None, beta=None, eps=1e-5, out=None):
         """LayerNorm over the last dimension of x: [rows, C] that keeps its row statistics -> (y, stats fp32 [rows, 2] = (mean, rstd)).
@@ -520,8 +531,9 @@ class Context:
         else:
             self._rows(out, "out", (rows, C))
         stats = torch.empty(rows, 2, dtype=torch.float32, device=self.torch_device)
-        self._check(self.lib.layer_norm_train(self.h, x.data_ptr(), self._ld(x, 0, C), out.data_ptr(), self._ld(out, 0, C), _addr(gamma), _addr(beta),
-                                              stats.data_ptr(), rows, C, eps), "layer_norm_train")
+        ldx, ldo = (x.stride(0), out.stride(0)) if rows > 1 else (C, C)
+        self._check(self.lib.layer_norm_train(self.h, x.data_ptr(), ldx, out.data_ptr(), ldo, _addr(gamma), _addr(beta), stats.data_ptr(), rows, C, eps),
+                    "layer_norm_train")
         return out, stats
 
     def layer_norm_backward(self, dy, x, stats, gamma=None, dx=None, need_weights=True):
@@ -543,12 +555,12 @@ class Context:
         dgamma = dbeta = ws = None
         nbytes = 0
         if need_weights:
-            dgamma = torch.empty(C, dtype=torch.float32, device=self.torch_device)
-            dbeta = torch.empty(C, dtype=torch.float32, device=self.torch_device)
+            dgamma, dbeta = torch.empty(2, C, dtype=torch.float32, device=self.torch_device).unbind(0)
             nbytes = self.lib.layer_norm_bwd_workspace(self.h, rows, C)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=self.torch_device) if nbytes else None
-        self._check(self.lib.layer_norm_bwd(self.h, dy.data_ptr(), self._ld(dy, 0, C), x.data_ptr(), self._ld(x, 0, C), stats.data_ptr(), _addr(gamma),
-                                            dx.data_ptr(), self._ld(dx, 0, C), _addr(dgamma), _addr(dbeta), rows, C, _addr(ws), nbytes), "layer_norm_bwd")
+        lddy, ldx, lddx = (dy.stride(0), x.stride(0), dx.stride(0)) if rows > 1 else (C, C, C)
+        self._check(self.lib.layer_norm_bwd(self.h, dy.data_ptr(), lddy, x.data_ptr(), ldx, stats.data_ptr(), _addr(gamma), dx.data_ptr(), lddx,
+                                            _addr(dgamma), _addr(dbeta), rows, C, _addr(ws), nbytes), "layer_norm_bwd")
         return dx, dgamma, dbeta
 
     def rel_buckets(self, num_buckets=32, max_distance=128, bidirectional=True):
