@@ -23,6 +23,7 @@ struct LnTrainParams {
   float* partial;                                 // backward: [gridDim.x][2][C] or null
   long long ldx, lddy, ldo;
   int rows, C, lpr;                               // lpr: lanes per row (unused in the WG form)
+  int stream;                                     // the output is larger than the caches: store past them
   float eps;
 };
 
@@ -35,9 +36,13 @@ STAR_DEV vec<T, 8> ln_load(const T* p, int n) {
   for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : from_f32<T>(0.f);
   return v;
 }
-template <class T, bool VEC>
+template <class T, bool VEC, bool STREAM>
 STAR_DEV void ln_store(T* p, vec<T, 8> v, int n) {
-  if constexpr (VEC) { *reinterpret_cast<vec<T, 8>*>(p) = v; return; }
+  if constexpr (VEC) {
+    if constexpr (STREAM) store_nt(reinterpret_cast<vec<T, 8>*>(p), v);
+    else *reinterpret_cast<vec<T, 8>*>(p) = v;
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) if (e < n) p[e] = v[e];
 }
@@ -113,6 +118,7 @@ ln_train_fwd_kernel(const LnTrainParams p) {
   if (!active) return;
   if (sub == 0 && p.stats) { p.stats[2 * row] = mean; p.stats[2 * row + 1] = rstd; }
   T* y = (T*)p.out + row * p.ldo;
+  auto write = [&](auto stream_tag) STAR_ALWAYS_INLINE {
 #pragma unroll
   for (int i = 0; i < CPL; ++i) {
     const int c = (sub + LPR * i) * 8;
@@ -123,9 +129,12 @@ ln_train_fwd_kernel(const LnTrainParams p) {
       vec<T, 8> o;
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = from_f32<T>((to_f32<T>(v[i][e]) - mean) * rstd * g[e] + b[e]);
-      ln_store<T, VEC>(y + c, o, p.C - c);
+      ln_store<T, VEC, decltype(stream_tag)::value>(y + c, o, p.C - c);
     }
   }
+  };
+  if (VEC && p.stream) write(std::integral_constant<bool, VEC>{});
+  else write(std::false_type{});
 }
 
 template <class T, bool VEC, int CPL, bool WG>
@@ -186,6 +195,7 @@ ln_train_bwd_kernel(const LnTrainParams p) {
     s2 = ln_row_sum<WG>(s2, LPR, sm, par * 2 + 1) * inv_c;
     if (!active) continue;
     T* dx = (T*)p.out + row * p.ldo;
+    auto write = [&](auto stream_tag) STAR_ALWAYS_INLINE {
 #pragma unroll
     for (int i = 0; i < CPL; ++i) {
       const int c = (sub + LPR * i) * 8;
@@ -198,9 +208,12 @@ ln_train_bwd_kernel(const LnTrainParams p) {
           const float xh = (to_f32<T>(vx[i][e]) - mean) * rstd;
           o[e] = from_f32<T>(rstd * (to_f32<T>(vd[i][e]) * g[e] - s1 - xh * s2));
         }
-        ln_store<T, VEC>(dx + c, o, p.C - c);
+        ln_store<T, VEC, decltype(stream_tag)::value>(dx + c, o, p.C - c);
       }
     }
+    };
+    if (VEC && p.stream) write(std::integral_constant<bool, VEC>{});
+    else write(std::false_type{});
   }
   if (!p.partial) return;
   float* part = p.partial + (size_t)blockIdx.x * 2 * p.C;
@@ -240,24 +253,24 @@ ln_train_bwd_kernel(const LnTrainParams p) {
   }
 }
 
-// dgamma | dbeta [2 C] from the partial rows: 32 columns per workgroup, eight threads per column share the rows, joined in a fixed order
+// dgamma | dbeta [2 C] from the partial rows: 16 columns per workgroup, sixteen threads per column share the rows, joined in a fixed order
 struct LnReduceParams { const float* partial; float* dgamma; float* dbeta; int C, parts; };
 STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256)
 ln_train_reduce_kernel(const LnReduceParams p) {
-  float* sm = reinterpret_cast<float*>(dyn_smem());                   // [8][32]
-  const int col = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + col, n = 2 * p.C;
+  float* sm = reinterpret_cast<float*>(dyn_smem());                   // [16][16]
+  const int col = threadIdx.x & 15, slice = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + col, n = 2 * p.C;
   float s = 0.f;
   if (c < n) {
 #pragma unroll 8
-    for (int r = slice; r < p.parts; r += 8) s += p.partial[(size_t)r * n + c];
+    for (int r = slice; r < p.parts; r += 16) s += p.partial[(size_t)r * n + c];
   }
-  sm[slice * 32 + col] = s;
+  sm[slice * 16 + col] = s;
   block_sync();
   if (slice || c >= n) return;
   float t = 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) t += sm[k * 32 + col];
+  for (int k = 0; k < 16; ++k) t += sm[k * 16 + col];
   if (c < p.C) { if (p.dgamma) p.dgamma[c] = t; }
   else if (p.dbeta) p.dbeta[c - p.C] = t;
 }

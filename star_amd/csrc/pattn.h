@@ -449,38 +449,49 @@ pattn_fwd_kernel(const PAttnParams p) {
   }
 }
 
-// joins the splits of a row, in their order: one wave per row, lane = d
+// joins the splits of a row, in their order: sixteen lanes per row, four values of d each
 template <class T>
 STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256)
 pattn_combine_kernel(const PAttnParams p) {
-  const int lane = threadIdx.x & 63;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int sub = threadIdx.x & 15;
   const int upb = p.heads / p.gp;
-  if (row >= (long long)p.batch * upb * p.rows) return;
+  const long long rows = (long long)p.batch * upb * p.rows;
+  const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (row >= rows) return;
   const int unit = (int)(row / p.rows), r = (int)(row - (long long)unit * p.rows);
   const float* base = p.part + ((size_t)unit * p.nsplit * p.rows + r) * PA_PART;
   const size_t step = (size_t)p.rows * PA_PART;
   const PRow rw = pa_row(p, r);
   const int b = unit / upb;
   // only the splits that had tiles wrote anything
-  const PRange rg = pa_range(p, b);
+  int n = p.kv_len ? p.kv_len[b] : p.Nk;
+  n = n < 0 ? 0 : n > p.Nk ? p.Nk : n;
+  int qs = p.q_start ? p.q_start[b] : p.start0;
+  qs = qs < -(1 << 29) ? -(1 << 29) : qs > 1 << 29 ? 1 << 29 : qs;
   const int blk = r / p.qb * p.qb, end = blk + p.qb - 1 < p.rows - 1 ? blk + p.qb - 1 : p.rows - 1;
-  const PTiles tl = pa_tiles(p, rg.n, rg.qs + pa_row(p, blk).i, rg.qs + pa_row(p, end).i);
-  const int need = wave_uniform((tl.na + tl.nb + p.per - 1) / p.per), ns = need < 1 ? 1 : need > p.nsplit ? p.nsplit : need;
+  const PTiles tl = pa_tiles(p, n, qs + pa_row(p, blk).i, qs + pa_row(p, end).i);
+  const int need = (tl.na + tl.nb + p.per - 1) / p.per, ns = need < 1 ? 1 : need > p.nsplit ? p.nsplit : need;
   float m = PA_NINF;
-  for (int s = lane; s < ns; s += 64) m = fmaxf(m, base[s * step + 64]);
-  m = wave_max(m);
-  float l = 0.f, o = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < ns; ++s) m = fmaxf(m, base[s * step + 64]);
+  float l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = 0; s < ns; ++s) {
     const float ms = base[s * step + 64];
     const float w = ms == PA_NINF ? 0.f : fast_exp2(ms - m);
+    const f32x4 v = *reinterpret_cast<const f32x4*>(base + s * step + 4 * sub);
     l += w * base[s * step + 65];
-    o += w * base[s * step + lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += w * v[e];
   }
   const int head = (unit - b * upb) * p.gp + rw.g;
-  ((T*)p.O)[(size_t)b * p.bso + (size_t)rw.i * p.ldo + head * 64 + lane] = from_f32<T>(l > 0.f ? o / l : l == 0.f ? 0.f : l);
-  if (p.lse && lane == 0) p.lse[((size_t)b * p.heads + head) * p.Nq + rw.i] = l == 0.f ? PA_NINF : (m + __builtin_log2f(l)) * PA_LN2;
+  const float mul = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+  vec<T, 4> out;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = from_f32<T>(o[e] * mul);
+  *reinterpret_cast<vec<T, 4>*>((T*)p.O + (size_t)b * p.bso + (size_t)rw.i * p.ldo + head * 64 + 4 * sub) = out;
+  if (p.lse && sub == 0) p.lse[((size_t)b * p.heads + head) * p.Nq + rw.i] = l == 0.f ? PA_NINF : (m + __builtin_log2f(l)) * PA_LN2;
 }
 
 }  // namespace star

@@ -61,7 +61,7 @@ constexpr int PA_SKEW = 48;                            // floats per row of the 
 
 // LDS past the tiles with a bias: table | a wave's sums by relative position, four arrays like the table | four skewed buffers
 template <class T, int BIAS, int COMP>
-STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256, 2)
+STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256, BIAS || COMP ? 2 : 3)
 pattn_dq_kernel(const PAttnParams p) {
   constexpr int NT = 256, QW = 32, QB = 4 * QW, PAD = PA_PAD_Q;
   char* smem = dyn_smem();                             // two buffers of (K tile | V tile)
@@ -165,11 +165,11 @@ pattn_dq_kernel(const PAttnParams p) {
   float lse_x = lse2;                                  // subtracted from the exponent: second walk less ex
 
   // one tile of 64 keys.  WALK 0: delta and the row sum, WALK 1: dS and dQ.  KIND 0: every row sees every key, the bias is one constant;
-  // 1: masks; 2: masks, the bias from the table, dS into the sums by relative position.  KIND 0: both halves' products come first, the second
-  // half's run beside the first half's vector work (the other kinds have no registers left for that)
+  // 1: masks; 2: masks, the bias from the table, dS into the sums by relative position.  With a bias (two waves per SIMD: the table's LDS) KIND 0 takes
+  // both halves' products first, the second half's run beside the first half's vector work; without, three waves per SIMD leave no registers for that
   auto body = [&](int k0, int bofs, bool masked, bool fl, float far, vec<T, 8>* ds, vec<T, 8>* dr, auto walk_tag, auto kind_tag) STAR_ALWAYS_INLINE {
     constexpr int WALK = decltype(walk_tag)::value, KIND = decltype(kind_tag)::value;
-    constexpr bool AHEAD = KIND == 0 && !COMP;
+    constexpr bool AHEAD = KIND == 0 && !COMP && BIAS;
     f32x16 s[2], dp[2];
     auto products = [&](int kb) STAR_ALWAYS_INLINE {
 #pragma unroll
