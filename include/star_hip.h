@@ -204,7 +204,7 @@ typedef struct star_pos_attn_desc {
   float scale;
   int32_t left, right;               /* window either way of the query's position; negative: no limit.  causal: right = 0 */
   int32_t sinks;                     /* the first `sinks` keys are visible past the left end of the window too */
-  int32_t num_buckets, bias_range;   /* bias_range <= 1024 */
+  int32_t num_buckets, bias_range;   /* at most 4096, at most 1024 */
   const int32_t* q_start; const int32_t* kv_len;              /* device int32 [batch] or null */
   const float* bias_table;           /* device fp32 [num_buckets][heads] or null: no bias */
   const int32_t* bias_buckets;       /* device int32 [2 * bias_range + 1] (star_rel_buckets), with the table */

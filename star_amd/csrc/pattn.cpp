@@ -8,6 +8,7 @@ namespace star {
 constexpr int PA_MAX_N = 1 << 28;         // queries and keys of a sequence
 constexpr int PA_MAX_LD = 1 << 23;        // elements: a tile's rows stay within 31 bits of bytes
 constexpr int PA_MAX_R = 1024;            // reach of the bias: its table and the sums by relative position live in LDS
+constexpr int PA_MAX_BUCKETS = 4096;      // a row block's sums by bucket go through the workspace
 constexpr int PA_NOLIM = 1 << 30;
 
 static bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -98,7 +99,7 @@ static int pa_check(Ctx* ctx, const PAttnArgs& a, const char* who) {
   if ((a.bsq | a.bsk | a.bsv | a.bso) & 7) return ctx->fail(w + "batch strides must be multiples of 8 elements");
   if (a.batch > 1 && (a.bsk == 0) != (a.bsv == 0)) return ctx->fail(w + "K and V are shared by the batch together or not at all");
   if ((a.table == nullptr) != (a.buckets == nullptr)) return ctx->fail(w + "the bias needs its table and its buckets");
-  if (a.table && (a.num_buckets < 1 || a.R < 0 || a.R > PA_MAX_R)) return ctx->fail(w + "the bias needs at least one bucket and a range of 0 .. 1024");
+  if (a.table && (a.num_buckets < 1 || a.num_buckets > PA_MAX_BUCKETS || a.R < 0 || a.R > PA_MAX_R)) return ctx->fail(w + "the bias needs 1 .. 4096 buckets and a range of 0 .. 1024");
   if (a.batch > 0 && a.Nq > 0 && (!a.Q || !al16(a.Q))) return ctx->fail(w + "Q is null or not 16-byte aligned");
   if (a.batch > 0 && a.Nk > 0 && (!a.K || !a.V || !al16(a.K) || !al16(a.V))) return ctx->fail(w + "K or V is null or not 16-byte aligned");
   return 0;
@@ -131,13 +132,13 @@ static bool pa_grid(PAttnParams& p, long long items, int units, dim3& grid) {
   return true;
 }
 
-// the backward pass's workspace: row statistics, sums of dS by relative position, parts of dK and dV
+// the backward pass's workspace: row statistics, sums of dS by bucket, parts of dK and dV
 struct PBwdLayout { size_t dsum, part, bytes; };
 static PBwdLayout pa_bwd_layout(const PAttnArgs& a, const PPlan& q, const PKPlan& k) {
   auto up = [](size_t n) { return (n + 15) & ~(size_t)15; };
   PBwdLayout l;
   l.dsum = up(3 * (size_t)q.units * q.rows * 4);
-  l.part = l.dsum + up(a.table ? (size_t)q.units * q.nblk * (2 * a.R + 1) * 4 : 0);
+  l.part = l.dsum + up(a.table ? (size_t)q.units * q.nblk * a.num_buckets * 4 : 0);
   l.bytes = l.part + k.part_slots * 128 * 128 * 4;
   return l;
 }
@@ -202,8 +203,8 @@ static int bwd_t(Ctx* ctx, PAttnParams p, const PPlan& q, const PKPlan& kp, floa
     }
   }
   if (BIAS) {
-    PDTableParams t{p.dsum, p.buckets, dtable, p.Nq > 0 ? p.batch : 0, p.heads, q.nblk, p.R, p.num_buckets};
-    STAR_LAUNCH(pattn_dtable_kernel, dim3((unsigned)p.heads), dim3(256), (size_t)R2 * 8 + (size_t)(R2 + 1) / 2 * 8 + 256 * 8, ctx->stream, t);
+    PDTableParams t{p.dsum, dtable, p.Nq > 0 ? p.batch : 0, p.heads, q.nblk, p.num_buckets};
+    STAR_LAUNCH(pattn_dtable_kernel, dim3((unsigned)p.heads), dim3(256), (size_t)(256 * 8), ctx->stream, t);
   }
   return 0;
 }

@@ -49,7 +49,7 @@ struct PAttnParams {
   float* part;                        // nsplit > 1: [unit][split][rows][68]: O[64], m, l
   // backward
   float* st_lse; float* st_delta; float* st_amax;      // [unit][rows]
-  float* dsum;                        // [item][2R + 1] sums of dS by relative position
+  float* dsum;                        // [unit][row block][num_buckets] sums of dS
   int sblk, split_s, split_n;         // dK / dV: the first sblk key blocks (those of the first tokens) in split_s parts each, the others in split_n
 };
 

@@ -312,8 +312,14 @@ pattn_dq_kernel(const PAttnParams p) {
     // entry i of the arrays belongs to j - p = i - R - PAD; what lies at +-R and past it joins the far tiles' sums
     auto column = [&](int i) { return (tab[RT + i] + tab[2 * RT + i]) + (tab[3 * RT + i] + tab[4 * RT + i]); };
     const int R2 = 2 * p.R + 1;
-    float* out = p.dsum + ((size_t)unit * p.nblk + qb) * R2;
-    for (int i = 1 + tid; i < R2 - 1; i += NT) out[i] = column(i + PAD);
+    float* rel = ends + 16;                            // [R2] sums by relative position, their buckets [R2], the threads' parts [256]
+    int* of = reinterpret_cast<int*>(rel + R2);
+    float* part = rel + 2 * R2;
+    for (int i = tid; i < R2; i += NT) {
+      const int c = p.buckets[i];
+      of[i] = c < 0 ? 0 : c >= p.num_buckets ? p.num_buckets - 1 : c;
+      if (i > 0 && i < R2 - 1) rel[i] = column(i + PAD);
+    }
     float e = 0.f;                                     // first wave: the columns up to -R; last wave: from R on (R = 0: past it)
     if (wv == 0) for (int i = lane; i <= PAD; i += 64) e += column(i);
     if (wv == 3) for (int i = lane; i <= PAD - (p.R == 0); i += 64) e += column(RT - 1 - i);
@@ -322,8 +328,27 @@ pattn_dq_kernel(const PAttnParams p) {
     block_sync();
     if (tid == 0) {
       const float left = ends[8] + ((ends[0] + ends[1]) + (ends[2] + ends[3])), right = ends[11] + ((ends[4] + ends[5]) + (ends[6] + ends[7]));
-      if (p.R > 0) { out[0] = left; out[R2 - 1] = right; }
-      else out[0] = left + right;
+      if (p.R > 0) { rel[0] = left; rel[R2 - 1] = right; }
+      else rel[0] = left + right;
+    }
+    block_sync();
+    // by bucket: its entries are shared out among `slices` threads, joined in a fixed order
+    float* out = p.dsum + ((size_t)unit * p.nblk + qb) * p.num_buckets;
+    int nb = 1;
+    while (nb < p.num_buckets && nb < NT) nb <<= 1;
+    const int slices = NT / nb, me = tid / nb;
+    for (int b0 = 0; b0 < p.num_buckets; b0 += nb) {
+      const int k = b0 + tid % nb;
+      float v = 0.f;
+#pragma unroll 4
+      for (int i = me; i < R2; i += slices) { const float x = rel[i]; v += of[i] == k ? x : 0.f; }
+      part[tid] = v;
+      block_sync();
+      if (me == 0 && k < p.num_buckets) {
+        for (int j = 1; j < slices; ++j) v += part[j * nb + tid];
+        out[k] = v;
+      }
+      block_sync();
     }
   }
 }
@@ -660,39 +685,30 @@ pattn_dkdv_join_kernel(const PAttnParams p) {
   }
 }
 
-// dtable[k][h]: the sums of a head's row blocks by relative position, in double and in a fixed order, then by bucket
-struct PDTableParams { const float* dsum; const int* buckets; float* dtable; int batch, heads, nblk, R, num_buckets; };
+// dtable[k][h]: the row blocks' sums of a head by bucket, in double and in a fixed order; the blocks are shared out among `slices` threads
+struct PDTableParams { const float* dsum; float* dtable; int batch, heads, nblk, num_buckets; };
 STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256)
 pattn_dtable_kernel(const PDTableParams p) {
-  const int h = blockIdx.x, R2 = 2 * p.R + 1;
-  double* rel = reinterpret_cast<double*>(dyn_smem());
-  int* of = reinterpret_cast<int*>(rel + R2);
-  for (int i = threadIdx.x; i < R2; i += 256) {
-    const int c = p.buckets[i];
-    of[i] = c < 0 ? 0 : c >= p.num_buckets ? p.num_buckets - 1 : c;
-    double s = 0.0;
-    for (int b = 0; b < p.batch; ++b) {
-      const float* d = p.dsum + ((size_t)b * p.heads + h) * p.nblk * R2 + i;
-#pragma unroll 4
-      for (int q = 0; q < p.nblk; ++q) s += (double)d[(size_t)q * R2];
-    }
-    rel[i] = s;
-  }
-  block_sync();
-  // a bucket's entries are shared out among `slices` threads, joined in a fixed order
+  double* part = reinterpret_cast<double*>(dyn_smem());               // [256]
+  const int h = blockIdx.x, tid = threadIdx.x;
+  const long long n = (long long)p.batch * p.nblk;
   int nb = 1;
   while (nb < p.num_buckets && nb < 256) nb <<= 1;
-  const int slices = 256 / nb, me = threadIdx.x / nb;
-  double* part = rel + R2 + (R2 + 1) / 2;              // [256], past the bucket numbers
-  for (int k0 = 0; k0 < p.num_buckets; k0 += nb) {
-    const int k = k0 + (int)threadIdx.x % nb;
+  const int slices = 256 / nb, me = tid / nb;
+  for (int b0 = 0; b0 < p.num_buckets; b0 += nb) {
+    const int k = b0 + tid % nb;
     double s = 0.0;
+    if (k < p.num_buckets) {
 #pragma unroll 4
-    for (int i = me; i < R2; i += slices) { const double v = rel[i]; s += of[i] == k ? v : 0.0; }
-    part[threadIdx.x] = s;
+      for (long long i = me; i < n; i += slices) {
+        const long long b = i / p.nblk;
+        s += (double)p.dsum[((size_t)(b * p.heads + h) * p.nblk + (i - b * p.nblk)) * p.num_buckets + k];
+      }
+    }
+    part[tid] = s;
     block_sync();
     if (me == 0 && k < p.num_buckets) {
-      for (int q = 1; q < slices; ++q) s += part[q * nb + threadIdx.x];
+      for (int j = 1; j < slices; ++j) s += part[j * nb + tid];
       p.dtable[(size_t)k * p.heads + h] = (float)s;
     }
     block_sync();

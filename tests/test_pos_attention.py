@@ -411,6 +411,7 @@ def test_refusals(backend, request):
         lambda: ctx.pos_attention(q, k, v, 4, 2, bias=(z(8, 2, dt=torch.float32), z(3, dt=i32))),
         lambda: ctx.pos_attention(q, k, v, 4, 2, bias=(z(8, 4), z(3, dt=i32))),
         lambda: ctx.pos_attention(q, k, v, 4, 2, bias=(z(0, 4, dt=torch.float32), z(3, dt=i32))),
+        lambda: ctx.pos_attention(q, k, v, 4, 2, bias=(z(4097, 4, dt=torch.float32), z(3, dt=i32))),
         lambda: ctx.pos_attention(q, k, v, 4, 2, bias=(z(8, 4, dt=torch.float32), z(4, dt=i32))),
         lambda: ctx.pos_attention(q, k, v, 4, 2, bias=(z(8, 4, dt=torch.float32), z(2051, dt=i32))),
         lambda: ctx.pos_attention(q, k, v, 4, 2, out=z(2, 8, 128)),
