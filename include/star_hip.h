@@ -47,7 +47,10 @@ enum { STAR_EPI_BIAS = 1, STAR_EPI_RES = 2, STAR_EPI_GEGLU = 4, STAR_EPI_OUT_F32
 int star_ctx_create(int device_id, int dtype, star_ctx** out);
 void star_ctx_destroy(star_ctx* ctx);
 const char* star_last_error(star_ctx* ctx);
-int star_set_stream(star_ctx* ctx, void* hip_stream);   /* use the caller's hipStream_t */
+int star_set_stream(star_ctx* ctx, void* hip_stream);   /* use the caller's hipStream_t; waits for what is queued on the one used so far
+                                                            (neither where one of the two is being captured into a graph) */
+int star_follow_stream(star_ctx* ctx, void* hip_stream);  /* the same without the wait where the context holds no scratch memory: for the entry
+                                                             points that take their workspace from the caller, on several streams in turn */
 int star_sync(star_ctx* ctx);
 int star_is_hostemu(void);                               /* 1 only in the test-tooling emulator build */
 int star_has_bench_variants(void);                       /* 1 only in builds with -DSTAR_BENCH_VARIANTS (tools/bench, emulator): losing A/B

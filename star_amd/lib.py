@@ -130,6 +130,7 @@ class Library:
         self.ctx_destroy = _sig(c, "star_ctx_destroy", None, vp)
         self.last_error = _sig(c, "star_last_error", ctypes.c_char_p, vp)
         self.set_stream = _sig(c, "star_set_stream", i32, vp, vp)
+        self.follow_stream = _sig(c, "star_follow_stream", i32, vp, vp)
         self.sync = _sig(c, "star_sync", i32, vp)
         self.pool_trim = _sig(c, "star_pool_trim", i32, vp)
         self.pool_bytes = _sig(c, "star_pool_bytes", sz, vp)
@@ -233,7 +234,7 @@ class Context:
                    6: "the device is not a gfx950 (MI355X) with the 160 KB LDS opt-in"}.get(rc, "")
             raise StarError(f"star_ctx_create failed (rc={rc}) {why}")
         self.h = h
-        self._stream = None             # what star_set_stream was last told
+        self._stream = None             # what star_set_stream / star_follow_stream was last told
         self.use_current_stream()
 
     def trim(self):
@@ -513,7 +514,7 @@ class Context:
             return
         s = _raw_stream(self.device_index)
         if s != self._stream:
-            self._check(self.lib.set_stream(self.h, s), "set_stream")
+            self._check(self.lib.follow_stream(self.h, s), "follow_stream")
             self._stream = s
 
     def layer_norm_train(self, x, gamma=None, beta=None, eps=1e-5, out=None):
