@@ -47,10 +47,10 @@ enum { STAR_EPI_BIAS = 1, STAR_EPI_RES = 2, STAR_EPI_GEGLU = 4, STAR_EPI_OUT_F32
 int star_ctx_create(int device_id, int dtype, star_ctx** out);
 void star_ctx_destroy(star_ctx* ctx);
 const char* star_last_error(star_ctx* ctx);
-int star_set_stream(star_ctx* ctx, void* hip_stream);   /* use the caller's hipStream_t; waits for what is queued on the one used so far
-                                                            (neither where one of the two is being captured into a graph) */
-int star_follow_stream(star_ctx* ctx, void* hip_stream);  /* the same without the wait where the context holds no scratch memory: for the entry
-                                                             points that take their workspace from the caller, on several streams in turn */
+int star_set_stream(star_ctx* ctx, void* hip_stream);   /* use the caller's hipStream_t */
+/* another stream for calls of the entry points that take their workspace from the caller (star_layer_norm_train / _bwd, star_pos_attn_fwd / _bwd)
+ * and nothing else: no wait, and *own (may be null) is the stream to set back in the same way before any other call. */
+int star_borrow_stream(star_ctx* ctx, void* hip_stream, void** own);
 int star_sync(star_ctx* ctx);
 int star_is_hostemu(void);                               /* 1 only in the test-tooling emulator build */
 int star_has_bench_variants(void);                       /* 1 only in builds with -DSTAR_BENCH_VARIANTS (tools/bench, emulator): losing A/B
@@ -197,6 +197,7 @@ int star_layer_norm_bwd(star_ctx* ctx, const void* dy, int64_t lddy, const void*
  * [0, Nk] and buckets outside [0, num_buckets) are clamped to it, q_start to +-2^29.  K and V rows that no query row of a 128-row block
  * (256 for long inputs) sees are not read; a NaN or an infinity in a V row (backward: also K, Q, dO rows) may reach the other rows of the
  * block that the row belongs to.  Sums are fp32; probabilities (and dS) are rounded to the 16-bit type for the second product.
+ * Outputs overlap neither each other nor an input (strided views of one buffer, a fused projection's, are fine).
  * The backward pass takes lse from the forward pass; gradients of heads, or of K and V, that are shared are sums over what shares them. */
 typedef struct star_pos_attn_desc {
   const void* Q; const void* K; const void* V; void* O;

@@ -113,20 +113,22 @@ void star_ctx_destroy(star_ctx* h) {
 }
 
 const char* star_last_error(star_ctx* h) { return h ? h->c.err.c_str() : "null ctx"; }
-// the arena hands freed blocks out again immediately on the assumption that all work is ordered on ONE stream: when the
-// caller moves to another stream, everything enqueued on the old one is drained first (rare: once per torch stream context).
-// Not where either is under capture: a stream under capture cannot be waited for, nor may a capture wait for what ran before it, and
-// what is captured runs later, in the order in which its graph is launched.
-static int move_stream(star_ctx* h, void* s, bool drain) {
-  if (h->c.stream != (hipStream_t)s && drain && !rt::stream_capturing((hipStream_t)s) && !rt::stream_capturing(h->c.stream)) {
-    DeviceScope scope(h->c.device);
+int star_set_stream(star_ctx* h, void* s) {
+  // the arena hands freed blocks out again immediately on the assumption that all work is ordered on ONE stream: when the
+  // caller moves to another stream, everything enqueued on the old one is drained first (rare: once per torch stream context)
+  if (h->c.stream != (hipStream_t)s) {
+    rt::set_device(h->c.device);
     if (rt::stream_sync(h->c.stream)) return h->c.fail(std::string("set_stream: sync of the previous stream failed: ") + rt::last_error_string());
   }
   h->c.stream = (hipStream_t)s;
   return 0;
 }
-int star_set_stream(star_ctx* h, void* s) { return h ? move_stream(h, s, true) : 1; }
-int star_follow_stream(star_ctx* h, void* s) { return h ? move_stream(h, s, h->c.pool.total() != 0) : 1; }
+int star_borrow_stream(star_ctx* h, void* s, void** own) {
+  if (!h) return 1;
+  if (own) *own = (void*)h->c.stream;
+  h->c.stream = (hipStream_t)s;
+  return 0;
+}
 int star_sync(star_ctx* h) {
   STAR_ENTER(h);
   if (rt::stream_sync(h->c.stream)) return h->c.fail(std::string("sync failed: ") + rt::last_error_string());

@@ -169,6 +169,7 @@ int op_pos_attn_fwd(Ctx* ctx, const PAttnArgs& a) {
   if (a.batch == 0 || a.Nq == 0) return 0;
   if (a.batch > 1 && a.bso == 0) return ctx->fail("pos_attn_fwd: the sequences' outputs lie on top of each other");
   if (!a.O || !al16(a.O)) return ctx->fail("pos_attn_fwd: O is null or not 16-byte aligned");
+  if (a.O == a.Q || (a.Nk > 0 && (a.O == a.K || a.O == a.V))) return ctx->fail("pos_attn_fwd: O must not be Q, K or V");
   const PPlan q = pa_plan(ctx, a, false);
   PAttnParams p = pa_params(a, q);
   const size_t need = pos_attn_workspace(ctx, a, false);
@@ -218,6 +219,14 @@ int op_pos_attn_bwd(Ctx* ctx, const PAttnArgs& a, float* dtable) {
   const bool any = a.batch > 0 && a.Nq > 0;
   if (any && (!a.dO || !a.dQ || !a.lse || !al16(a.dO) || !al16(a.dQ))) return ctx->fail("pos_attn_bwd: dO, dQ or lse is null or not 16-byte aligned");
   if (a.batch > 0 && a.Nk > 0 && (!a.dK || !a.dV || !al16(a.dK) || !al16(a.dV))) return ctx->fail("pos_attn_bwd: dK or dV is null or not 16-byte aligned");
+  const void* in[4] = {any ? a.Q : nullptr, any ? a.dO : nullptr, a.K, a.V};
+  const void* gr[3] = {any ? a.dQ : nullptr, a.Nk > 0 ? a.dK : nullptr, a.Nk > 0 ? a.dV : nullptr};
+  for (int i = 0; i < 3; ++i) {
+    bool twice = false;
+    for (int j = 0; j < 4; ++j) twice = twice || (gr[i] && gr[i] == in[j]);
+    for (int j = 0; j < i; ++j) twice = twice || (gr[i] && gr[i] == gr[j]);
+    if (twice) return ctx->fail("pos_attn_bwd: dQ, dK and dV must not be each other or one of the inputs");
+  }
   const bool shared = a.bsk == 0 && a.bsv == 0;
   if (a.batch > 1 && ((a.Nq > 0 && a.bsdq == 0) || (!shared && a.Nk > 0 && (a.bsdk == 0 || a.bsdv == 0))))
     return ctx->fail("pos_attn_bwd: the sequences' gradients lie on top of each other");

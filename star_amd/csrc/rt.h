@@ -17,7 +17,6 @@ inline int memcpy_d2d(void* d, const void* s, size_t n, hipStream_t) { memcpy(d,
 inline int stream_sync(hipStream_t) { return 0; }
 inline int set_device(int) { return 0; }
 inline int get_device() { return 0; }
-inline bool stream_capturing(hipStream_t) { return false; }
 inline int device_count() { return 1; }
 inline bool device_is_gfx950(int) { return true; }
 inline int device_cu_count(int) { return 256; }
@@ -50,13 +49,6 @@ inline int memcpy_d2d(void* d, const void* s, size_t n, hipStream_t st) { return
 inline int stream_sync(hipStream_t s) { return hipStreamSynchronize(s) != hipSuccess; }
 inline int set_device(int d) { return hipSetDevice(d) != hipSuccess; }
 inline int get_device() { int d = -1; return hipGetDevice(&d) == hipSuccess ? d : -1; }
-// whether work on the stream is being captured into a graph (the null stream cannot be)
-inline bool stream_capturing(hipStream_t s) {
-  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-  if (!s) return false;
-  if (hipStreamIsCapturing(s, &st) != hipSuccess) { (void)hipGetLastError(); return false; }
-  return st != hipStreamCaptureStatusNone;
-}
 inline int device_count() { int n = 0; if (hipGetDeviceCount(&n) != hipSuccess) return 0; return n; }
 inline const char* last_error_string() { return hipGetErrorString(hipGetLastError()); }
 inline bool device_is_gfx950(int d) {

@@ -130,7 +130,7 @@ class Library:
         self.ctx_destroy = _sig(c, "star_ctx_destroy", None, vp)
         self.last_error = _sig(c, "star_last_error", ctypes.c_char_p, vp)
         self.set_stream = _sig(c, "star_set_stream", i32, vp, vp)
-        self.follow_stream = _sig(c, "star_follow_stream", i32, vp, vp)
+        self.borrow_stream = _sig(c, "star_borrow_stream", i32, vp, vp, ctypes.POINTER(vp))
         self.sync = _sig(c, "star_sync", i32, vp)
         self.pool_trim = _sig(c, "star_pool_trim", i32, vp)
         self.pool_bytes = _sig(c, "star_pool_bytes", sz, vp)
@@ -234,7 +234,7 @@ class Context:
                    6: "the device is not a gfx950 (MI355X) with the 160 KB LDS opt-in"}.get(rc, "")
             raise StarError(f"star_ctx_create failed (rc={rc}) {why}")
         self.h = h
-        self._stream = None             # what star_set_stream / star_follow_stream was last told
+        self._stream = None             # what star_set_stream was last told
         self.use_current_stream()
 
     def trim(self):
@@ -508,14 +508,19 @@ class Context:
             raise StarError(f"a row stride of {ld} elements is too large")
         return ld
 
-    def _follow_stream(self):
-        """torch's current stream on this device becomes the context's (a call of its own only where it changed)"""
-        if self.lib.is_hostemu:
-            return
-        s = _raw_stream(self.device_index)
-        if s != self._stream:
-            self._check(self.lib.follow_stream(self.h, s), "follow_stream")
-            self._stream = s
+    def _launch(self, fn, what, *args):
+        """a call on torch's current stream of this device; the context's own stream stays what it was for the other calls"""
+        s = None if self.lib.is_hostemu else _raw_stream(self.device_index)
+        if s == self._stream:
+            rc = fn(self.h, *args)
+        else:
+            own = ctypes.c_void_p()
+            self._check(self.lib.borrow_stream(self.h, s, ctypes.byref(own)), "borrow_stream")
+            try:
+                rc = fn(self.h, *args)
+            finally:
+                self.lib.borrow_stream(self.h, own, None)
+        self._check(rc, what)
 
     def layer_norm_train(self, x, gamma=None, beta=None, eps=1e-5, out=None):
         """LayerNorm over the last dimension of x: [rows, C] that keeps its row statistics -> (y, stats fp32 [rows, 2] = (mean, rstd)).
@@ -526,15 +531,14 @@ class Context:
         rows, C = x.shape
         self._vec_f32(gamma, C, "gamma")
         self._vec_f32(beta, C, "beta")
-        self._follow_stream()
         if out is None:
             out = torch.empty(rows, C, dtype=self.dtype, device=self.torch_device)
         else:
             self._rows(out, "out", (rows, C))
         stats = torch.empty(rows, 2, dtype=torch.float32, device=self.torch_device)
         ldx, ldo = (x.stride(0), out.stride(0)) if rows > 1 else (C, C)
-        self._check(self.lib.layer_norm_train(self.h, x.data_ptr(), ldx, out.data_ptr(), ldo, _addr(gamma), _addr(beta), stats.data_ptr(), rows, C, eps),
-                    "layer_norm_train")
+        self._launch(self.lib.layer_norm_train, "layer_norm_train", x.data_ptr(), ldx, out.data_ptr(), ldo, _addr(gamma), _addr(beta), stats.data_ptr(),
+                     rows, C, eps)
         return out, stats
 
     def layer_norm_backward(self, dy, x, stats, gamma=None, dx=None, need_weights=True):
@@ -548,7 +552,6 @@ class Context:
         if not stats.is_contiguous():
             raise StarError("stats must be contiguous")
         self._vec_f32(gamma, C, "gamma")
-        self._follow_stream()
         if dx is None:
             dx = torch.empty(rows, C, dtype=self.dtype, device=self.torch_device)
         else:
@@ -560,8 +563,8 @@ class Context:
             nbytes = self.lib.layer_norm_bwd_workspace(self.h, rows, C)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=self.torch_device) if nbytes else None
         lddy, ldx, lddx = (dy.stride(0), x.stride(0), dx.stride(0)) if rows > 1 else (C, C, C)
-        self._check(self.lib.layer_norm_bwd(self.h, dy.data_ptr(), lddy, x.data_ptr(), ldx, stats.data_ptr(), _addr(gamma), dx.data_ptr(), lddx,
-                                            _addr(dgamma), _addr(dbeta), rows, C, _addr(ws), nbytes), "layer_norm_bwd")
+        self._launch(self.lib.layer_norm_bwd, "layer_norm_bwd", dy.data_ptr(), lddy, x.data_ptr(), ldx, stats.data_ptr(), _addr(gamma), dx.data_ptr(),
+                     lddx, _addr(dgamma), _addr(dbeta), rows, C, _addr(ws), nbytes)
         return dx, dgamma, dbeta
 
     def rel_buckets(self, num_buckets=32, max_distance=128, bidirectional=True):
@@ -640,7 +643,6 @@ class Context:
         -> [B, Nq, heads*64], with return_lse also log sum exp of the scores, fp32 [B, heads, Nq].  A row that sees no key: 0 and -inf."""
         d = self._pos_desc(q, k, v, heads, kv_heads, scale, window, sinks, causal, q_start, kv_len, bias)
         B, Nq = q.shape[:2]
-        self._follow_stream()
         if out is None:
             out = torch.empty(B, Nq, heads * 64, dtype=self.dtype, device=self.torch_device)
         else:
@@ -649,7 +651,7 @@ class Context:
         lse = torch.empty(B, heads, Nq, dtype=torch.float32, device=self.torch_device) if return_lse else None
         d.lse = lse.data_ptr() if lse is not None else None
         ws = self._pos_workspace(d, False)      # held until the call is queued
-        self._check(self.lib.pos_attn_fwd(self.h, ctypes.byref(d)), "pos_attn_fwd")
+        self._launch(self.lib.pos_attn_fwd, "pos_attn_fwd", ctypes.byref(d))
         del ws
         return (out, lse) if return_lse else out
 
@@ -665,7 +667,6 @@ class Context:
             raise StarError("lse must be contiguous")
         if B > 1 and k.shape[0] == B and k.numel() and d.bsk == 0:
             raise StarError("k and v are expanded over the batch: pass them as [1, Nk, ...], their gradients are sums over the batch")
-        self._follow_stream()
         dq, dk, dv = (torch.empty(t.shape, dtype=self.dtype, device=self.torch_device) if g is None else g for t, g in ((q, dq), (k, dk), (v, dv)))
         g = PosAttnGrads()
         for t, like, what in ((dq, q, "dq"), (dk, k, "dk"), (dv, v, "dv")):
@@ -678,7 +679,7 @@ class Context:
         dtable = torch.empty(d.num_buckets, heads, dtype=torch.float32, device=self.torch_device) if bias is not None else None
         g.dbias_table = dtable.data_ptr() if dtable is not None else None
         ws = self._pos_workspace(d, True)
-        self._check(self.lib.pos_attn_bwd(self.h, ctypes.byref(d), ctypes.byref(g)), "pos_attn_bwd")
+        self._launch(self.lib.pos_attn_bwd, "pos_attn_bwd", ctypes.byref(d), ctypes.byref(g))
         del ws
         return dq, dk, dv, dtable
 

@@ -122,6 +122,15 @@ def test_bias_of_one_bucket_range_zero(backend, request):
     run_case(ctx, q, k, v, do, 1, 1, bias=(torch.tensor([[0.7]]), [0]))
 
 
+@pytest.mark.parametrize("Nq,Nk,start", [(140, 1300, 1100), (200, 200, 0), (1, 2500, 2400)])
+def test_the_largest_bias(backend, Nq, Nk, start, request):
+    """the longest reach and the most buckets; a kernel's table then takes the greater part of the shared memory"""
+    g = torch.Generator().manual_seed(Nk)
+    q, k, v, do, _ = inputs(torch.float16, 1, Nq, Nk, 1, 1, 31)
+    bias = (torch.randn(4096, 1, generator=g), torch.randint(0, 4096, (2049,), generator=g).tolist())
+    run_case(ctx_of(backend, torch.float16, request), q, k, v, do, 1, 1, q_start=[start], bias=bias)
+
+
 STEPS = [
     (3, 1, 700, 4, 1, {"kv_len": [700, 65, 1], "causal": True}),
     (2, 1, 1500, 2, 2, {"kv_len": [1500, 900], "window": (300, 0), "sinks": 4}),
@@ -430,6 +439,21 @@ def test_refusals(backend, request):
     assert torch.equal(ctx.pos_attention(q, k, v, 4, 2), ok[0])
 
 
+def test_outputs_on_top_of_inputs_are_refused(backend, request):
+    ctx = ctx_of(backend, torch.float16, request)
+    q, k, v = (torch.randn(2, 9, 128).half().to(ctx.torch_device) for _ in range(3))
+    out, lse = ctx.pos_attention(q, k, v, 2, return_lse=True)
+    ref = ctx.pos_attention_backward(out, q, k, v, lse, 2)
+    for t in (q, k, v):
+        with pytest.raises(L.StarError, match="must not be"):
+            ctx.pos_attention(q, k, v, 2, out=t)
+    for kw in ({"dq": q}, {"dq": out}, {"dk": k}, {"dv": q}, {"dk": ref[2], "dv": ref[2]}, {"dq": ref[1], "dk": ref[1]}):
+        with pytest.raises(L.StarError, match="must not be"):
+            ctx.pos_attention_backward(out, q, k, v, lse, 2, **kw)
+    again = ctx.pos_attention_backward(out, q, k, v, lse, 2)
+    assert all(torch.equal(a, b) for a, b in zip(ref[:3], again[:3]))
+
+
 def test_refusals_of_the_c_entry_points(backend, request):
     ctx = ctx_of(backend, torch.float16, request)
     dev = ctx.torch_device
@@ -565,6 +589,35 @@ def test_another_stream_and_two_at_once():
             outs.append((ctx.pos_attention(*b, 8, 2), rb))
     torch.cuda.synchronize()
     assert all(torch.equal(o, r) for o, r in outs)
+
+
+def test_the_own_stream_stays(backend, request):
+    """a call on another stream leaves the context's own one as it was for the calls that do not follow torch's; refused calls too"""
+    ctx = ctx_of(backend, torch.float16, request)
+    own, seen = ctypes.c_void_p(), ctypes.c_void_p()
+    assert ctx.lib.borrow_stream(None, None, None)
+
+    def own_stream():
+        assert ctx.lib.borrow_stream(ctx.h, None, ctypes.byref(seen)) == 0 and ctx.lib.borrow_stream(ctx.h, seen, None) == 0
+        return seen.value
+
+    before = own_stream()
+    x = torch.randn(70, 64).half().to(ctx.torch_device)
+    ref = ctx.layer_norm_train(x)
+    if backend == "emu":
+        assert ctx.lib.borrow_stream(ctx.h, 4096, ctypes.byref(own)) == 0 and own.value == before and own_stream() == 4096
+        assert ctx.lib.borrow_stream(ctx.h, own, None) == 0
+        return
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        y = ctx.layer_norm_train(x)
+        assert own_stream() == before
+        with pytest.raises(L.StarError):
+            ctx.pos_attention(x[None], x[None], x[None], 1, out=x[None])
+    assert own_stream() == before
+    s.synchronize()
+    assert torch.equal(y[0], ref[0]) and torch.equal(y[1], ref[1])
 
 
 @pytest.mark.gpu
