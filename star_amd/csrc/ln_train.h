@@ -4,7 +4,9 @@
 //   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), xh = (x - mu) r, y = xh gamma + beta        stats[row] = (mu, r)
 //   a = dy gamma, dx = r (a - mean(a) - xh mean(a xh)),  dgamma = sum_rows dy xh,  dbeta = sum_rows dy
 //
-// Both passes move every row once (forward 4 bytes per element, backward 6) and are bound by HBM.  A row is held in registers as it
+// Both passes move every row once (forward 4 bytes per element, backward 6) and are bound by HBM: f16, 843 264 x 320 forward 199 us = 5.4 TB/s,
+// 214 272 x 640 backward 197 us = 4.2 TB/s, where a copy of 2 GiB runs at 4.9.  A few hundred rows are the latency of the launches:
+// 154 x 1024 forward 4 us, 616 x 1024 backward 8 us + 3 us for the sums.  (The next row's loads ahead of this one's sums lost: 207 -> 262 us.)  A row is held in registers as it
 // was read (16-bit, four registers per 16-byte chunk), the two moments are taken from it there: one read, no second pass over memory.
 // LPR lanes share a row (the least power of two that holds it in CPL chunks per lane, at least eight where the row has eight chunks,
 // so that a group reads whole 128-byte lines); rows past 64 x CPL chunks take a whole workgroup (WG).

@@ -16,8 +16,13 @@
 // COMP: as in the forward pass, dS and P with what their rounding left, for short rows.
 // Key blocks that many rows see (those of the first tokens: every row), or few blocks on many compute units, are dealt to several
 // workgroups along the rows; each writes its part in fp32, pattn_dkdv_join_kernel adds the parts in their order.
-// Per 32 x 32 block and wave both kernels read 12 - 16 KB of LDS against 12 - 16 matrix instructions of 32 cycles: LDS bandwidth and the
-// vector work on the scores (about 36 cycles a score) are what bounds them.
+// What bounds them: no one unit.  bf16, 2 x 4099 tokens, 16 heads, a bias: 1.0 ms (traced dQ 0.59, dK / dV 0.50 ms); 10 d flops a pair make
+// about 0.33 PFLOP/s, 0.6 with the products that are taken again (18 d).  Counters of the dQ kernel: vector unit busy 49 % of the cycles, matrix
+// unit 30 %, waves waiting 29 %, at 1.9 GHz.  Timed without its DMA, its exponentials or its last products (in copies, results wrong) each kernel
+// loses 6 - 10 %: what is left is the chain product -> exponential -> pack -> product of one tile, of two waves per SIMD.  Short sequences (4 x
+// 226 tokens, 16 heads: 35 + 21 + 5 us) are one such chain after the other and a launch each.  A window of 1024 over 4500 tokens, 16 heads in
+// groups of 4: 171 us (dQ 80, dK / dV 89, join 9 traced), 0.26 PFLOP/s.  Tried and no faster: 64 rows per wave in dQ (spills), three waves per
+// SIMD with a bias, halves of a tile in step with each other, the transposed fragments read before the exponentials.
 #pragma once
 #include "pattn.h"
 

@@ -489,7 +489,7 @@ class Context:
             self._chk_tensor(t, dtype or self.dtype)
         if shape is not None and t.shape != shape:
             raise StarError(f"{what} must be {list(shape)}, got {list(t.shape)}")
-        if t.stride(-1) != 1 and t.numel() and t.shape[-1] > 1:
+        if t.dim() == 0 or (t.stride(-1) != 1 and t.numel() and t.shape[-1] > 1):
             raise StarError(f"{what} must have unit stride in its last dimension")
 
     def _vec_f32(self, t, n, what):

@@ -217,6 +217,8 @@ def test_refusals(backend, request):
         lambda: ctx.layer_norm_train(x.bfloat16()),
         lambda: ctx.layer_norm_train(x.float()),
         lambda: ctx.layer_norm_train(x[None]),
+        lambda: ctx.layer_norm_train(x[0, 0]),
+        lambda: ctx.layer_norm_train([1.0]),
         lambda: ctx.layer_norm_train(x.t()),
         lambda: ctx.layer_norm_train(x, gamma.half()),
         lambda: ctx.layer_norm_train(x, gamma[:32]),
