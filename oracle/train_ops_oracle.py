@@ -65,9 +65,11 @@ def bucket_scheme(num_buckets, distance, bidirectional):
     return out
 
 
-def pos_attention(q, k, v, heads, kv_heads, scale, left=-1, right=-1, sinks=0, q_start=None, kv_len=None, bias=None, dout=None):
+def pos_attention(q, k, v, heads, kv_heads, scale, left=-1, right=-1, sinks=0, q_start=None, kv_len=None, bias=None, dout=None, tight=False):
     """q [B, Nq, heads*64], k, v [B or 1, Nk, kv_heads*64] (any float type) -> dict of 64-bit out, lse and, with dout, dq, dk, dv, dtable;
-    `tol_*` beside each: the elementwise bound for the inputs' type."""
+    `tol_*` beside each: the elementwise bound for the inputs' type.
+    tight: f16's absolute half step for dS by rows and key blocks.  A kernel rounds 2^e dS with max|dP| 2^e >= 2^13, the maximum over what the row
+    sees (dq) or over the rows of the 64-row tiles that see some of the 128 keys of a block (dk): a half step is then 2^-25 2^-13 max|dP|."""
     T = q.dtype
     u = half_step(T)
     sub = 2.0 ** -25 if T == torch.float16 else 0.0          # f16's absolute half step below its normal range
@@ -85,8 +87,10 @@ def pos_attention(q, k, v, heads, kv_heads, scale, left=-1, right=-1, sinks=0, q
         if bias is not None:
             r["dtable"], r["tol_dtable"] = torch.zeros(bias[0].shape, dtype=F), torch.zeros(bias[0].shape, dtype=F)
         biggest = float(DO.abs().max()) if DO.numel() else 0.0
+    step, oks = torch.zeros(B, heads, Nq, dtype=F), []
     for b in range(B):
         ok, rel = visible(Nq, Nk, left, right, sinks, None if q_start is None else q_start[b], None if kv_len is None else kv_len[b])
+        oks.append(ok)
         seen = ok.any(1, keepdim=True)
         if bias is not None:
             R = (len(bias[1]) - 1) // 2
@@ -128,15 +132,30 @@ def pos_attention(q, k, v, heads, kv_heads, scale, left=-1, right=-1, sinks=0, q
             rS = u * dS.abs() + eS * (1 + u)
             top = float(g.abs().max()) if g.numel() else 0.0
             r["dq"][b, :, h] = scale * (dS @ kh)
-            r["tol_dq"][b, :, h] = u * r["dq"][b, :, h].abs() + abs(scale) * (rS @ kh.abs() + sub * top * kh.abs().sum(0)) + sub + 1e-30
+            least = sub * top * kh.abs().sum(0)
+            if tight:
+                step[b, h] = sub * 2.0 ** -13 * (dp.abs() * ok).amax(1)
+                least = step[b, h][:, None] * (ok.to(F) @ kh.abs())
+            r["tol_dq"][b, :, h] = u * r["dq"][b, :, h].abs() + abs(scale) * (rS @ kh.abs() + least) + sub + 1e-30
             kvh = h // G
             r["dk"][b % S, :, kvh] += scale * (dS.T @ qh)
-            r["tol_dk"][b % S, :, kvh] += abs(scale) * (rS.T @ qh.abs() + sub * biggest * qh.abs().sum(0)) + Nq * U32 * abs(scale) * (dS.abs().T @ qh.abs())
+            r["tol_dk"][b % S, :, kvh] += abs(scale) * (rS.T @ qh.abs() + (0.0 if tight else sub * biggest * qh.abs().sum(0))) + Nq * U32 * abs(scale) * (dS.abs().T @ qh.abs())
             r["dv"][b % S, :, kvh] += P.T @ g
             r["tol_dv"][b % S, :, kvh] += (u + Nq * U32) * (P.T @ g.abs()) + (ep * P).T @ g.abs() + sub * 2.0 ** -10 * g.abs().sum(0)
             if bias is not None:
                 r["dtable"][:, h].index_add_(0, which.flatten(), dS.flatten())
                 r["tol_dtable"][:, h].index_add_(0, which.flatten(), (eS + (Nq + Nk) * U32 * dS.abs()).flatten())
+    if dout is not None and tight:
+        for j in range(0, Nk, 128):
+            blk = slice(j, j + 128)
+            # the tokens that see some of these keys, and those that may share a tile of 64 rows with them
+            near = [torch.nn.functional.max_pool1d(o[:, blk].any(1).to(F)[None, None], 127, 1, 63)[0, 0] for o in oks]
+            for b in range(B):
+                for kvh in range(kv_heads):
+                    same = range(B) if S == 1 else [b]
+                    most = max(float((step[c, kvh * G:(kvh + 1) * G] * near[c]).max()) for c in same)
+                    for h in range(kvh * G, (kvh + 1) * G):
+                        r["tol_dk"][b % S, blk, kvh] += abs(scale) * most * (oks[b][:, blk].to(F).T @ Q[b, :, h].abs())
     if dout is not None:
         for n in ("dk", "dv"):
             r["tol_" + n] += u * r[n].abs() + sub + 1e-30

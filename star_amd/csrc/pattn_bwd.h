@@ -11,8 +11,9 @@
 // delta is not taken as rowsum(dO O): O is rounded to 16 bits and comes from rounded P, and where a softmax is peaked dP - delta is a small
 // difference -- the error of dQ and dK would be several times their own rounding.  The first walk costs 8 of 36 matrix instructions
 // per 32 x 32 block.  dP is the same sum in the same order in both kernels, so that a row with one visible key has dS = 0 exactly.
-// f16 only: P and dS are scaled by powers of two before they are rounded, so that long rows and small gradients do not fall
-// below f16's normal range: P by 2^10 (P <= 1), dS by the largest |dO| of the row (dQ) or of the rows walked so far (dK).
+// f16 only: P and dS are scaled by powers of two before they are rounded, so that they neither leave f16's range nor fall below its
+// normal one: P by 2^10 (P <= 1), dS by the largest |dP| among the row's visible keys (dQ), which the first walk keeps, or among those of the
+// rows walked so far (dK): P <= 1 and |dP - delta| <= 2 max |dP| bound it, whatever the sizes of dO and V.
 // COMP: as in the forward pass, dS and P with what their rounding left, for short rows.
 // Key blocks that many rows see (those of the first tokens: every row), or few blocks on many compute units, are dealt to several
 // workgroups along the rows; each writes its part in fp32, pattn_dkdv_join_kernel adds the parts in their order.
@@ -28,25 +29,17 @@
 
 namespace star {
 
-// 2^e with |x| 2^e in [8, 16): the exponent as an integer, 0 for zero and non-finite x; within [-24, 40]
+// 2^e with |x| 2^e in [2^13, 2^14), so that twice that is below f16's 65504: the exponent as an integer, 0 for zero and non-finite x.  x is a sum
+// of 64 products of f16 values, which lies between 2^-48 and 2^38: e within [-40, 60], and so is 2^(e - e') for two of them
+constexpr int PA_EXP_MAX = 60;
 STAR_DEV int pa_fit_exp(float x) {
   const uint32_t ex = (__builtin_bit_cast(uint32_t, x) >> 23) & 255u;
-  if (ex == 0u) return x == 0.f ? 0 : 40;
+  if (ex == 0u) return x == 0.f ? 0 : PA_EXP_MAX;
   if (ex == 255u) return 0;
-  const int e = 130 - (int)ex;
-  return e < -24 ? -24 : e > 40 ? 40 : e;
+  const int e = 140 - (int)ex;
+  return e < -40 ? -40 : e > PA_EXP_MAX ? PA_EXP_MAX : e;
 }
 STAR_DEV float pa_pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
-
-template <class T>
-STAR_DEV float pa_absmax(const vec<T, 8>* f) {
-  float m = 0.f;
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = fmaxf(m, __builtin_fabsf(to_f32<T>(f[ks][e])));
-  return m;
-}
 
 // hi + lo += x, lo gathers what the additions to hi rounded away
 STAR_DEV void pa_add2(float& hi, float& lo, float x) {
@@ -114,13 +107,8 @@ pattn_dq_kernel(const PAttnParams p) {
   const int hi = pa_hi(p, n, pos), lo0 = pa_lo(p, pos), lo = lo0;
   const int lo_c = lo0 < hi ? lo0 : hi;
   const bool sole = hi - lo_c + (p.sinks < lo_c ? p.sinks : lo_c) == 1;        // the row sees one key: P = 1
-  float exf = 0.f, ipw = 1.f;                          // f16: dS is rounded as 2^ex dS; ex and 2^-ex
-  if constexpr (__is_same(T, f16)) {
-    const float amax = pair_max(pa_absmax<T>(gf));
-    const int ex = pa_fit_exp(amax);
-    exf = (float)ex; ipw = pa_pow2(-ex);
-    if (row_ok && h2 == 0) p.st_amax[(size_t)unit * p.rows + row] = amax;
-  }
+  constexpr bool FIT = __is_same(T, f16);              // dS is rounded as 2^ex dS: 2^ex and 2^-ex, known after the first walk
+  float pw = 1.f, ipw = 1.f, amax = 0.f;               // amax: the largest |dP| of the visible keys
   float delta = 0.f, lsum = 0.f, delta_lo = 0.f, lsum_lo = 0.f, far_l = 0.f, far_r = 0.f;
   float sum_l = 0.f, sum_r = 0.f;                      // dS of far tiles: keys at -R or before, at R or past it; what the adds rounded away
   float low_l = 0.f, low_r = 0.f;
@@ -167,7 +155,6 @@ pattn_dq_kernel(const PAttnParams p) {
   for (int c2 = 0; c2 < 2; ++c2)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[c2][r] = 0.f;
-  float lse_x = lse2;                                  // subtracted from the exponent: second walk less ex
 
   // one tile of 64 keys.  WALK 0: delta and the row sum, WALK 1: dS and dQ.  KIND 0: every row sees every key, the bias is one constant;
   // 1: masks; 2: masks, the bias from the table, dS into the sums by relative position.  With a bias (two waves per SIMD: the table's LDS) KIND 0 takes
@@ -188,7 +175,7 @@ pattn_dq_kernel(const PAttnParams p) {
       }
     };
     if constexpr (AHEAD) { products(0); products(1); }
-    const float off = far - lse_x;
+    const float off = far - lse2;
     float t0 = 0.f, t1 = 0.f, l0 = 0.f, l1 = 0.f;        // this tile's sums
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
@@ -197,22 +184,23 @@ pattn_dq_kernel(const PAttnParams p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int j = (r & 3) + 8 * (r >> 2), key = k0 + kb * 32 + j + 4 * h2;
-        float x = __builtin_fmaf(s[kb][r], p.c, KIND == 2 ? tab[at + j] - lse_x : off);
+        float x = __builtin_fmaf(s[kb][r], p.c, KIND == 2 ? tab[at + j] - lse2 : off);
         bool see = true;
         if constexpr (KIND != 0) {
           see = !masked | ((key < hi) & ((key >= lo) | (key < p.sinks)));
-          x = sole ? (WALK ? exf : 0.f) : x;
+          x = sole ? 0.f : x;
         }
         float pr = fast_exp2(x);
         if constexpr (KIND != 0) pr = see ? pr : 0.f;
         if constexpr (WALK == 0) {
           const float d = KIND != 0 ? (see ? dp[kb][r] : 0.f) : dp[kb][r];
+          if constexpr (FIT) amax = fmaxf(amax, __builtin_fabsf(d));
           if (r & 1) { l1 += pr; t1 = __builtin_fmaf(pr, d, t1); }
           else { l0 += pr; t0 = __builtin_fmaf(pr, d, t0); }
         } else {
           // (subtracted at the end: a row with one visible key has dP - delta = 0 exactly, and sums that start at -delta cost the table's
           // gradient half of its digits past 1e-6)
-          float v = pr * (dp[kb][r] - delta);
+          float v = pr * (FIT ? __builtin_fmaf(dp[kb][r], pw, -delta) : dp[kb][r] - delta);
           if constexpr (KIND != 0) v = see ? v : 0.f;
           T hi16, lo16{};
           pa_round<T, COMP>(v, hi16, lo16);
@@ -295,11 +283,17 @@ pattn_dq_kernel(const PAttnParams p) {
     const float l = pair_sum(lsum + lsum_lo), d = pair_sum(delta + delta_lo);
     delta = l > 0.f ? d / l : l == 0.f ? 0.f : l;
     if (l > 0.f) lse2 += __builtin_log2f(l);
-    lse_x = lse2 - exf;
+    if constexpr (FIT) amax = pair_max(amax);
     if (row_ok && h2 == 0) {
       const size_t at = (size_t)unit * p.rows + row;
       p.st_lse[at] = lse2;
       p.st_delta[at] = delta;
+      if constexpr (FIT) p.st_amax[at] = amax;
+    }
+    if constexpr (FIT) {
+      const int ex = pa_fit_exp(amax);
+      pw = pa_pow2(ex); ipw = pa_pow2(-ex);
+      delta *= pw;                                     // (a power of two: dP 2^ex - delta 2^ex is as exact as dP - delta)
     }
   }
   for (int it = 0; it < total; ++it, buf ^= 1) {
@@ -444,7 +438,7 @@ pattn_dkdv_kernel(const PAttnParams p) {
     first = all * sl.part / sl.parts; last = all * (sl.part + 1) / sl.parts;
   }
   long long done = 0;                                  // tiles before the current head's
-  int E = 40;                                          // f16: dK is summed as 2^E dK
+  int E = PA_EXP_MAX;                                          // f16: dK is summed as 2^E dK
   for (int w = 0; w < nb * subs; ++w) {
     const int b = shared ? wave_uniform(w / subs) : kb0, sub = shared ? w - b * subs : w;
     const int head0 = kvh * G + sub * p.gp, unit = b * upb + kvh * subs + sub;

@@ -1,0 +1,95 @@
+"""Position-dependent attention (star_pos_attn_fwd / _bwd) at the ends of its inputs' range: large and small V and dO, large scores and biases,
+against the formulas in 64 bits; bounds as in test_pos_attention.py, f16's absolute half steps by rows and key blocks (`tight`)."""
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "oracle"))
+import train_ops_oracle as O  # noqa: E402
+from util import BACKENDS, DTYPES, make_ctx  # noqa: E402
+
+
+@pytest.fixture(params=BACKENDS)
+def backend(request):
+    return request.param
+
+
+def ctx_of(backend, dtype, request):
+    return make_ctx(backend, dtype, request.getfixturevalue("emu_lib") if backend == "emu" else None)
+
+
+def randn(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+def within(got, ref, tol, what):
+    got = got.detach().cpu().double()
+    assert got.shape == ref.shape and torch.isfinite(got).all(), what
+    over = (got - ref).abs() - tol
+    assert float(over.max()) <= 0, f"{what}: off by {float(over.max()):.3g} more than its bound, largest value {float(ref.abs().max()):.3g}"
+
+
+def check_backward(ctx, q, k, v, do, H, KH, *, window=(-1, -1), sinks=0, scale=0.125, bias=None):
+    dev = ctx.torch_device
+    kw = dict(scale=scale, window=window, sinks=sinks)
+    if bias is not None:
+        kw["bias"] = (bias[0].to(dev), torch.tensor(bias[1], dtype=torch.int32, device=dev))
+    ref = O.pos_attention(q, k, v, H, KH, scale, *window, sinks, bias=bias, dout=do, tight=True)
+    a = [t.to(dev) for t in (q, k, v)]
+    _, lse = ctx.pos_attention(*a, H, KH, return_lse=True, **kw)
+    got = dict(zip(("dq", "dk", "dv", "dtable"), ctx.pos_attention_backward(do.to(dev), *a, lse, H, KH, **kw)))
+    for n, t in got.items():
+        if t is not None:
+            within(t, ref[n], ref["tol_" + n], n)
+
+
+def bias_of(with_bias, H, seed):
+    return (randn(seed, 16, H), O.bucket_scheme(16, 30, True)) if with_bias else None
+
+
+# ------------------------------------------------------------------------------------------------------ sizes of V and dO
+# N, window: a row sees two keys, a row sees a few dozen, and more keys than the span up to which the remainders of P and dS are kept
+SPANS = [(40, (1, 0)), (150, (20, 20)), (600, (-1, -1))]
+LARGE_V = [("aligned", 200.0, 1e-2), ("aligned", 500.0, 1e-4), ("aligned", 1000.0, 1e-5), ("channel", 8000.0, 1e-2), ("channel", 20000.0, 1e-4)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("N,window", SPANS)
+@pytest.mark.parametrize("form,size,grad", LARGE_V)
+def test_large_values_with_small_gradients(backend, dtype, N, window, with_bias, form, size, grad, request):
+    """V rows of one sign and a common size, or one channel far above the others, with gradients that keep the results finite: dP = dO V^T passes
+    f16's range relative to dO by far.  q and k are small beside `scale`, so that dq and dk are numbers of a normal size"""
+    q, k = (2.0 ** -4 * randn(n, 1, N, 64) for n in (1, 2))
+    do = grad * (1 + 0.3 * randn(3, 1, N, 64))
+    if form == "aligned":
+        v = size * torch.sign(randn(4, 1, N, 1)).expand(1, N, 64) * (1 + 0.01 * randn(5, 1, N, 64))
+    else:
+        v = randn(4, 1, N, 64)
+        v[:, :, 5] = (size * v[:, :, 5]).clamp(-60000, 60000)
+    check_backward(ctx_of(backend, dtype, request), *(t.to(dtype) for t in (q, k, v, do)), 1, 1, window=window, scale=32.0, bias=bias_of(with_bias, 1, 6))
+
+
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("N,window", SPANS)
+@pytest.mark.parametrize("size,grad", [(1.0, 2.0 ** -12), (1.0, 2.0 ** -18), (1e-3, 2.0 ** -10)])
+def test_small_gradients_keep_their_digits(backend, N, window, with_bias, size, grad, request):
+    """dS below f16's normal range, dq and dk inside it: scale k and scale q are large"""
+    q, k = (2.0 ** -10 * randn(n, 1, N, 64) for n in (1, 2))
+    v, do = size * randn(4, 1, N, 64), grad * randn(3, 1, N, 64)
+    check_backward(ctx_of(backend, torch.float16, request), *(t.half() for t in (q, k, v, do)), 1, 1, window=window, scale=2.0 ** 17, bias=bias_of(with_bias, 1, 7))
+
+
+@pytest.mark.parametrize("H,KH", [(1, 1), (4, 2)])
+@pytest.mark.parametrize("turned", [False, True])
+def test_rows_of_different_sizes(backend, H, KH, turned, request):
+    """rows whose dO differ by 2^12, far apart along the sequence: each row's dq, and dk of the keys that only small rows see, keep their digits"""
+    N = 500
+    q, k = 2.0 ** -10 * randn(1, 1, N, H * 64), 2.0 ** -10 * randn(2, 1, N, KH * 64)
+    v, do = randn(4, 1, N, KH * 64), 2.0 ** -4 * randn(3, 1, N, H * 64)
+    do[:, 250:] *= 2.0 ** -12
+    if turned:
+        do = do.flip(1)
+    check_backward(ctx_of(backend, torch.float16, request), *(t.half() for t in (q, k, v, do)), H, KH, window=(20, 20), scale=2.0 ** 17)
