@@ -159,20 +159,22 @@ ln_train_bwd_kernel(const LnTrainParams p) {
   for (long long it = blockIdx.x; it < steps; it += gridDim.x, par ^= 1) {
     const long long row = WG ? it : it * rpb + wave * rpw + lane / LPR;
     const bool active = row < p.rows;
-    const long long rr = active ? row : p.rows - 1;
-    const T* x = (const T*)p.x + rr * p.ldx;
-    const T* dy = (const T*)p.dy + rr * p.lddy;
-    const float mean = p.stats[2 * rr], rstd = p.stats[2 * rr + 1];
+    // a row past the end is all zeros: it adds nothing to the sums, and it reads no row that its owner may be writing (dx may be x or dy)
+    const T* x = (const T*)p.x + row * p.ldx;
+    const T* dy = (const T*)p.dy + row * p.lddy;
+    float mean = 0.f, rstd = 0.f;
+    if (active) { mean = p.stats[2 * row]; rstd = p.stats[2 * row + 1]; }
     vec<T, 8> vx[CPL], vd[CPL];
 #pragma unroll
     for (int i = 0; i < CPL; ++i) {
       const int c = (sub + LPR * i) * 8;
       if (c < p.C) {
-        vx[i] = ln_load<T, VEC>(x + c, p.C - c);
-        vd[i] = ln_load<T, VEC>(dy + c, p.C - c);
-        if (!active) {                                                // a row past the end adds nothing to the sums
+        if (active) {
+          vx[i] = ln_load<T, VEC>(x + c, p.C - c);
+          vd[i] = ln_load<T, VEC>(dy + c, p.C - c);
+        } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) vd[i][e] = from_f32<T>(0.f);
+          for (int e = 0; e < 8; ++e) { vx[i][e] = from_f32<T>(0.f); vd[i][e] = from_f32<T>(0.f); }
         }
       }
     }

@@ -241,3 +241,20 @@ def test_refusals(backend, request):
     assert ctx.lib.layer_norm_train(ctx.h, None, 64, x.data_ptr(), 64, None, None, None, 4, 64, 1e-5)
     assert ctx.lib.layer_norm_train(None, x.data_ptr(), 64, x.data_ptr(), 64, None, None, None, 4, 64, 1e-5)
     assert ctx.lib.layer_norm_train(ctx.h, x.data_ptr(), 64, x.data_ptr(), 64, None, None, None, -1, 64, 1e-5)
+
+
+@pytest.mark.parametrize("rows,C", [(1, 8), (3, 50), (5, 320), (3, 1024)])
+def test_in_place_where_the_gradient_leaves_the_range(backend, rows, C, request):
+    """dx overflows to infinity and is written over x or dy: the weight's gradients, finite numbers, are those of the call with an output of its own"""
+    ctx = ctx_of(backend, torch.float16, request)
+    dev = ctx.torch_device
+    x = torch.randn(rows, C, generator=torch.Generator().manual_seed(1)).half().to(dev)
+    dy = (6e4 * torch.sign(torch.randn(rows, C, generator=torch.Generator().manual_seed(2)))).half().to(dev)
+    gamma = torch.full((C,), 1e4, device=dev)
+    _, st = ctx.layer_norm_train(x, gamma)
+    dx, dg, db = ctx.layer_norm_backward(dy, x, st, gamma)
+    assert torch.isinf(dx).any(1).all() and torch.isfinite(dg).all() and torch.isfinite(db).all()
+    for target in ("x", "dy"):
+        xc, dyc = x.clone(), dy.clone()
+        got, g2, b2 = ctx.layer_norm_backward(dyc, xc, st, gamma, dx=xc if target == "x" else dyc)
+        assert torch.equal(got, dx) and torch.equal(g2, dg) and torch.equal(b2, db), target
