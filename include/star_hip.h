@@ -172,7 +172,7 @@ int star_layer_norm_rowab_from_partials(star_ctx* ctx, const float* ln_partial, 
 /* nn.LayerNorm in training (what fine-tuning the norms of the blocks above needs, video_super_resolution/scripts/train_sr.py:648-731):
  * the forward pass that keeps its row statistics, and the backward pass.  x, y, dy, dx: rows in the context's 16-bit type; gamma, beta and
  * their gradients fp32 [C], null for a norm without them; any C up to 16384, any row strides >= C (multiples of 8 with 16-byte aligned
- * pointers take the fast path).  y may be x, and dx may be x or dy.
+ * pointers take the fast path).  y may be x, and dx may be x or dy, with the same row stride; otherwise outputs overlap no input.
  *   stats[row] = (mean, 1 / sqrt(var + eps)), fp32 pairs (null: not kept)
  *   dx = rstd (a - mean(a) - xh mean(a xh)), a = dy gamma;  dgamma = sum_rows dy xh;  dbeta = sum_rows dy  (either may be null)
  * The row sums go through a workspace of star_layer_norm_bwd_workspace() bytes (none where both are null) that the caller owns and

@@ -86,6 +86,7 @@ int op_layer_norm_train(Ctx* ctx, const void* x, long long ldx, void* y, long lo
   if (rows == 0) return 0;
   if (!x || !y) return ctx->fail("layer_norm_train: null tensor");
   if (ldx < C || ldy < C) return ctx->fail("layer_norm_train: row strides must be at least C");
+  if (y == x && rows > 1 && ldy != ldx) return ctx->fail("layer_norm_train: y over x needs x's row stride");
   ProfScope ps(ctx, PK_LN, 0.0, 4.0 * rows * (double)C);
   const bool v = !((C | ldx | ldy) & 7) && al16(x) && al16(y) && al16(gamma) && al16(beta);
   const LnShape sh = ln_shape(C, v, false);
@@ -103,6 +104,7 @@ int op_layer_norm_bwd(Ctx* ctx, const void* dy, long long lddy, const void* x, l
   if (rows > 0) {
     if (!dy || !x || !dx || !stats) return ctx->fail("layer_norm_bwd: null tensor");
     if (ldx < C || lddy < C || lddx < C) return ctx->fail("layer_norm_bwd: row strides must be at least C");
+    if (rows > 1 && ((dx == x && lddx != ldx) || (dx == dy && lddx != lddy))) return ctx->fail("layer_norm_bwd: dx over x or dy needs its row stride");
     const bool v = !((C | ldx | lddy | lddx) & 7) && al16(x) && al16(dy) && al16(dx) && al16(gamma);
     const LnShape sh = ln_shape(C, v, true);
     blocks = ln_bwd_blocks(ctx, rows, sh.lpr);

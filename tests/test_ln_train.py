@@ -258,3 +258,21 @@ def test_in_place_where_the_gradient_leaves_the_range(backend, rows, C, request)
         xc, dyc = x.clone(), dy.clone()
         got, g2, b2 = ctx.layer_norm_backward(dyc, xc, st, gamma, dx=xc if target == "x" else dyc)
         assert torch.equal(got, dx) and torch.equal(g2, dg) and torch.equal(b2, db), target
+
+
+def test_in_place_with_another_row_stride_is_refused(backend, request):
+    """rows of y would lie over rows of x that are still to be read"""
+    ctx = ctx_of(backend, torch.float16, request)
+    dev = ctx.torch_device
+    buf = torch.randn(16, 64, generator=torch.Generator().manual_seed(1)).half().to(dev)
+    keep = buf.clone()
+    wide, flat = buf.reshape(8, 128)[:, :64], buf[:8]
+    st = ctx.layer_norm_train(wide)[1]
+    other = torch.zeros(8, 64, dtype=torch.float16, device=dev)
+    for x, y in ((wide, flat), (flat, wide)):
+        for call in (lambda: ctx.layer_norm_train(x, out=y), lambda: ctx.layer_norm_backward(other, x, st, dx=y), lambda: ctx.layer_norm_backward(x, other, st, dx=y)):
+            with pytest.raises(L.StarError, match="row stride"):
+                call()
+    assert torch.equal(buf, keep)
+    one = ctx.layer_norm_train(wide[:1])[0]                                  # (of one row the stride says nothing)
+    assert torch.equal(ctx.layer_norm_train(wide[:1], out=flat[:1])[0], one)
