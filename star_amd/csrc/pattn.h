@@ -12,8 +12,10 @@
 //     than 1.5 x their own rounding): the scale, the bias and the running maximum meet in one fma per score.
 //   * A tile is "plain" when every row of the workgroup sees all of its keys and the bias is one constant there (past +-R it is: the far
 //     tiles, nearly all of a long sequence).  Plain tiles take the lazy path: P = exp2(fma(s, c, off)) against the running maximum as it
-//     stands, the row sum as overflow probe.  Every other tile, and every tile until each row of the wave has seen one, takes the
-//     exact path: masks and bias per score, the tile's maximum, rescale.  Tiles that no row of the workgroup sees are not visited.
+//     stands, the row sum as overflow probe.  Every other tile, every tile until each row of the wave has seen one, and every tile of a wave
+//     with a maximum past 2^12 (base 2) takes the exact path: masks and bias per score, the tile's maximum, rescale.  Past that a score's
+//     own rounding, which the exact path's maximum has and one fma with it has not, is no longer small: equal scores would weigh differently from
+//     tile to tile.  Tiles that no row of the workgroup sees are not visited.
 //   * Rows of the heads that share a K / V head are packed token-major into one workgroup's rows (GP of them), so that a group reads its
 //     keys once; with a bias a workgroup keeps to one head (one table column in LDS).
 //   * K / V rows that no row of the workgroup sees are staged as zeros through the descriptor's range check: what lies behind kv_len or
@@ -62,6 +64,7 @@ constexpr int PA_KT = 64, PA_TILE = PA_KT * 128;       // keys per tile, bytes o
 constexpr int PA_PART = 68;                            // floats per row of a split's partial result (16-byte rows)
 constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
 constexpr float PA_NINF = -__builtin_inff();
+constexpr float PA_LARGE = 4096.0f;                    // of scores in base 2: half a step of fp32 there is a relative 1.7e-4 of exp2
 
 struct PRange { int n, qs; };                          // keys in hand, position of row 0 -- both clamped to what the kernels can index
 STAR_DEV PRange pa_range(const PAttnParams& p, int b) {
@@ -292,7 +295,7 @@ pattn_fwd_kernel(const PAttnParams p) {
   float m_run[NQ], l_run[NQ];                          // base 2; m = -inf: the row has seen no key yet
 #pragma unroll
   for (int qi = 0; qi < NQ; ++qi) { m_run[qi] = PA_NINF; l_run[qi] = 0.f; }
-  bool fresh = true;                                   // wave-uniform: some row may not have seen a key yet
+  bool fresh = true;                                   // wave-uniform: some row may not have seen a key yet, or its maximum is large
 
   auto tile = [&](int it, int buf) STAR_ALWAYS_INLINE {
     const int k0 = tile_of(it) * PA_KT;
@@ -390,7 +393,7 @@ pattn_fwd_kernel(const PAttnParams p) {
         for (int db = 0; db < 2; ++db)
 #pragma unroll
           for (int r = 0; r < 16; ++r) oacc[qi][db][r] *= alpha;
-        unseen = unseen || m_new == PA_NINF;
+        unseen = unseen || !(__builtin_fabsf(m_new) <= PA_LARGE);
         expo(qi, 1.f, m_new == PA_NINF ? 0.f : -m_new);
       }
       fresh = wave_any(unseen);

@@ -93,3 +93,27 @@ def test_rows_of_different_sizes(backend, H, KH, turned, request):
     if turned:
         do = do.flip(1)
     check_backward(ctx_of(backend, torch.float16, request), *(t.half() for t in (q, k, v, do)), H, KH, window=(20, 20), scale=2.0 ** 17)
+
+
+# ----------------------------------------------------------------------------------------------------- large scores and biases
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Nq", [1, 130])
+@pytest.mark.parametrize("score,bias", [(1e6, None), (-1e6, None), (1e9, None), (-1e9, None), (3e5, -2e6), (3e4, 5e5)])
+def test_equal_scores_weigh_the_same(backend, dtype, Nq, score, bias, request):
+    """every score is the same large number, whatever it rounds to: the output is the mean of V.  P is 1 for each key, its sum exact: rounded are the
+    output and, twice at most, its terms' products with 1 (fp32 sums of 700 terms beside that)"""
+    ctx = ctx_of(backend, dtype, request)
+    dev = ctx.torch_device
+    N = 700
+    q, k = torch.ones(1, Nq, 64).to(dtype), torch.full((1, N, 64), 0.75).to(dtype)
+    v = randn(3, 1, N, 64).to(dtype)
+    kw = {}
+    if bias is not None:
+        kw["bias"] = (torch.full((16, 1), bias, device=dev), ctx.rel_buckets(16, 30))
+    out, lse = ctx.pos_attention(q.to(dev), k.to(dev), v.to(dev), 1, scale=score / 48.0, return_lse=True, **kw)
+    ref = v.double().mean(1, keepdim=True).expand(1, Nq, 64)
+    u = O.half_step(dtype)
+    within(out, ref, u * ref.abs() + 710 * O.U32 * v.double().abs().mean(1, keepdim=True) + (2.0 ** -25 if dtype == torch.float16 else 0), "out")
+    # the score: 64 products, the scale, the base and back, and log 700 added to it
+    total = score + (bias or 0.0)
+    within(lse, torch.full((1, 1, Nq), total + 6.551080335).double(), torch.full((1, 1, Nq), 80 * O.U32 * (abs(score) + abs(bias or 0.0))).double(), "lse")
