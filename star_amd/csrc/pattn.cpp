@@ -137,7 +137,7 @@ struct PBwdLayout { size_t dsum, part, bytes; };
 static PBwdLayout pa_bwd_layout(const PAttnArgs& a, const PPlan& q, const PKPlan& k) {
   auto up = [](size_t n) { return (n + 15) & ~(size_t)15; };
   PBwdLayout l;
-  l.dsum = up(3 * (size_t)q.units * q.rows * 4);
+  l.dsum = up(4 * (size_t)q.units * q.rows * 4);
   l.part = l.dsum + up(a.table ? (size_t)q.units * q.nblk * a.num_buckets * 4 : 0);
   l.bytes = l.part + k.part_slots * 128 * 128 * 4;
   return l;
@@ -196,7 +196,7 @@ static int bwd_t(Ctx* ctx, PAttnParams p, const PPlan& q, const PKPlan& kp, floa
     PAttnParams k = p;
     k.nblk = kp.slots; k.sblk = kp.sblk; k.split_s = kp.split_s; k.split_n = kp.split_n;
     if (!pa_grid(k, (long long)kp.units * kp.slots, kp.units, grid)) return ctx->fail("pos_attn_bwd: too many workgroups");
-    const size_t smem = 2 * (2 * PA_TILE + 64 * 12 + 16) + (BIAS ? (size_t)(R2 + 2 * PA_PAD_K) * 4 : 0);
+    const size_t smem = 2 * (2 * PA_TILE + PA_ROWB) + (BIAS ? (size_t)(R2 + 2 * PA_PAD_K) * 4 : 0);
     STAR_LAUNCH((pattn_dkdv_kernel<T, BIAS, COMP>), grid, dim3(256), smem, ctx->stream, k);
     if (kp.part_slots) {
       const long long blocks = (long long)kp.units * (kp.split_n > 1 ? kp.nblk : kp.sblk);
@@ -239,7 +239,7 @@ int op_pos_attn_bwd(Ctx* ctx, const PAttnArgs& a, float* dtable) {
   const PKPlan kp = pa_kplan(ctx, a, q);
   const PBwdLayout l = pa_bwd_layout(a, q, kp);
   const size_t st = (size_t)q.units * q.rows;
-  p.st_lse = (float*)a.workspace; p.st_delta = p.st_lse + st; p.st_amax = p.st_delta + st;
+  p.st_ref = (float*)a.workspace; p.st_log = p.st_ref + st; p.st_delta = p.st_log + st; p.st_amax = p.st_delta + st;
   p.dsum = (float*)((char*)a.workspace + l.dsum);
   p.part = (float*)((char*)a.workspace + l.part);
   ProfScope ps(ctx, PK_ATTN_SELF, 0.0, 0.0, a.batch, a.heads, a.Nq, a.Nk);

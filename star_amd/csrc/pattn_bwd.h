@@ -5,9 +5,12 @@
 //
 // Two kernels, so that every sum has one owner and a fixed order (no atomics): the same call gives the same bits.
 //   pattn_dq_kernel    a wave owns query rows and walks the keys twice.  First walk: delta, and the log-sum-exp once more (the caller's is
-//                      rounded to fp32 and in base e).  Second walk: dS, dQ, and the sums of dS by relative position.
+//                      rounded to fp32 and in base e), as two numbers: the row's reference point, and log2 of the sum relative to it.  Second walk:
+//                      dS, dQ, and the sums of dS by relative position.
 //   pattn_dkdv_kernel  a wave owns 32 keys and walks the query rows of every head of the group (and of every sequence, where the batch
 //                      shares K and V): dK, dV.
+// The reference is the caller's log-sum-exp; for a wave with one past 2^12 (base 2), whose roundings are no small factors of exp2, it is the row's maximum,
+// found anew in the first walk, and each score is rounded as in the forward pass before the reference is subtracted.
 // delta is not taken as rowsum(dO O): O is rounded to 16 bits and comes from rounded P, and where a softmax is peaked dP - delta is a small
 // difference -- the error of dQ and dK would be several times their own rounding.  The first walk costs 8 of 36 matrix instructions
 // per 32 x 32 block.  dP is the same sum in the same order in both kernels, so that a row with one visible key has dS = 0 exactly.
@@ -55,6 +58,7 @@ STAR_DEV void pa_round(float v, T& hi, T& lo) {
   if constexpr (COMP) lo = from_f32<T>(v - to_f32<T>(hi));
 }
 
+constexpr int PA_ROWB = 64 * 20 + 16;                  // dK / dV: bytes of a tile's row statistics
 constexpr int PA_SKEW = 48;                            // floats per row of the skewed buffer: 16 keys + 32 rows - 1 diagonals, and one to spare
 
 // LDS past the tiles with a bias: table | a wave's sums by relative position, four arrays like the table | four skewed buffers
@@ -103,7 +107,10 @@ pattn_dq_kernel(const PAttnParams p) {
     }
   }
   const float lse_in = p.lse[((size_t)b * p.heads + head0 + rw.g) * p.Nq + rw.i];
-  float lse2 = !row_ok || lse_in == PA_NINF ? -PA_NINF : lse_in * PA_LOG2E;
+  const bool dead = !row_ok || lse_in == PA_NINF;      // P = 0
+  float ref = dead ? -PA_NINF : lse_in * PA_LOG2E, ll = 0.f;   // P = exp2(y - ref - ll), y the score in base 2
+  const bool large = wave_any(!dead && !(__builtin_fabsf(ref) <= PA_LARGE));
+  if (large) ref = PA_NINF;                            // (the running maximum)
   const int hi = pa_hi(p, n, pos), lo0 = pa_lo(p, pos), lo = lo0;
   const int lo_c = lo0 < hi ? lo0 : hi;
   const bool sole = hi - lo_c + (p.sinks < lo_c ? p.sinks : lo_c) == 1;        // the row sees one key: P = 1
@@ -156,8 +163,9 @@ pattn_dq_kernel(const PAttnParams p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[c2][r] = 0.f;
 
-  // one tile of 64 keys.  WALK 0: delta and the row sum, WALK 1: dS and dQ.  KIND 0: every row sees every key, the bias is one constant;
-  // 1: masks; 2: masks, the bias from the table, dS into the sums by relative position.  With a bias (two waves per SIMD: the table's LDS) KIND 0 takes
+  // one tile of 64 keys.  WALK 0: delta and the row sum, 2: the same with the maximum (large rows, KIND 2 or 3), 1: dS and dQ.  KIND 0: every row sees
+  // every key, the bias is one constant; 1: masks; 2: masks, the bias from the table, dS into the sums by relative position; 3: large rows, masks,
+  // the bias one constant.  With a bias (two waves per SIMD: the table's LDS) KIND 0 takes
   // both halves' products first, the second half's run beside the first half's vector work; without, three waves per SIMD leave no registers for that
   auto body = [&](int k0, int bofs, bool masked, bool fl, float far, vec<T, 8>* ds, vec<T, 8>* dr, auto walk_tag, auto kind_tag) STAR_ALWAYS_INLINE {
     constexpr int WALK = decltype(walk_tag)::value, KIND = decltype(kind_tag)::value;
@@ -175,28 +183,51 @@ pattn_dq_kernel(const PAttnParams p) {
       }
     };
     if constexpr (AHEAD) { products(0); products(1); }
-    const float off = far - lse2;
+    const float off = (far - ref) - ll;
     float t0 = 0.f, t1 = 0.f, l0 = 0.f, l1 = 0.f;        // this tile's sums
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       if constexpr (!AHEAD) { STAR_SCHED_FENCE(); products(kb); }
       const int at = k0 + kb * 32 + 4 * h2 - pos + p.R + PAD;                  // the table's entry of the lane's first key
+      float base = 0.f;                                  // WALK 2: the maximum, 0 while there is none
+      if constexpr (WALK == 2) {
+        float mx = PA_NINF;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = (r & 3) + 8 * (r >> 2), key = k0 + kb * 32 + j + 4 * h2;
+          const float y = __builtin_fmaf(s[kb][r], p.c, KIND == 2 ? tab[at + j] : far);
+          s[kb][r] = !masked | ((key < hi) & ((key >= lo) | (key < p.sinks))) ? y : PA_NINF;
+          mx = fmaxf(mx, s[kb][r]);
+        }
+        const float m_new = fmaxf(ref, pair_max(mx));
+        const float f = m_new == PA_NINF ? 1.f : fast_exp2(ref - m_new);
+        ref = m_new;
+        base = m_new == PA_NINF ? 0.f : m_new;
+        lsum *= f; lsum_lo *= f; delta *= f; delta_lo *= f;
+        t0 *= f; t1 *= f; l0 *= f; l1 *= f;
+      }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int j = (r & 3) + 8 * (r >> 2), key = k0 + kb * 32 + j + 4 * h2;
-        float x = __builtin_fmaf(s[kb][r], p.c, KIND == 2 ? tab[at + j] - lse2 : off);
+        float x;
+        if constexpr (WALK == 2) x = s[kb][r] - base;
+        else if constexpr (KIND >= 2) {
+          x = __builtin_fmaf(s[kb][r], p.c, KIND == 2 ? tab[at + j] : far) - ref;
+          if constexpr (WALK == 1) x -= ll;
+        } else x = __builtin_fmaf(s[kb][r], p.c, off);
         bool see = true;
         if constexpr (KIND != 0) {
           see = !masked | ((key < hi) & ((key >= lo) | (key < p.sinks)));
-          x = sole ? 0.f : x;
+          if constexpr (WALK == 1) x = sole ? 0.f : x;
         }
         float pr = fast_exp2(x);
         if constexpr (KIND != 0) pr = see ? pr : 0.f;
-        if constexpr (WALK == 0) {
+        if constexpr (WALK != 1) {
           const float d = KIND != 0 ? (see ? dp[kb][r] : 0.f) : dp[kb][r];
           if constexpr (FIT) amax = fmaxf(amax, __builtin_fabsf(d));
-          if (r & 1) { l1 += pr; t1 = __builtin_fmaf(pr, d, t1); }
-          else { l0 += pr; t0 = __builtin_fmaf(pr, d, t0); }
+          const float wt = KIND != 0 && sole ? 1.f : pr; // (delta is dP itself, whatever the last bit of P)
+          if (r & 1) { l1 += pr; t1 = __builtin_fmaf(wt, d, t1); }
+          else { l0 += pr; t0 = __builtin_fmaf(wt, d, t0); }
         } else {
           // (subtracted at the end: a row with one visible key has dP - delta = 0 exactly, and sums that start at -delta cost the table's
           // gradient half of its digits past 1e-6)
@@ -227,7 +258,7 @@ pattn_dq_kernel(const PAttnParams p) {
         }
       }
     }
-    if constexpr (WALK == 0) {
+    if constexpr (WALK != 1) {
       // (with a bias to 2^-48: what delta is off by stays in the sums over millions of pairs that make up the table's gradient)
       if constexpr (BIAS) { pa_add2(lsum, lsum_lo, l0 + l1); pa_add2(delta, delta_lo, t0 + t1); }
       else { lsum += l0 + l1; delta += t0 + t1; }
@@ -250,8 +281,17 @@ pattn_dq_kernel(const PAttnParams p) {
       far = fl ? far_l : far_r;
     }
     vec<T, 8> ds[4], dr[4];                            // 2^ex dS, sixteen keys each, and what its rounding left
-    if (BIAS && near) body(k0, bofs, masked, fl, far, ds, dr, walk_tag, std::integral_constant<int, BIAS ? 2 : 1>{});
-    else if (masked) body(k0, bofs, masked, fl, far, ds, dr, walk_tag, std::integral_constant<int, 1>{});
+    using K1 = std::integral_constant<int, 1>;
+    using K2 = std::integral_constant<int, BIAS ? 2 : 3>;
+    using K3 = std::integral_constant<int, 3>;
+    using W2 = std::integral_constant<int, 2>;
+    if (decltype(walk_tag)::value == 0 && large) {
+      if (near) body(k0, bofs, masked, fl, far, ds, dr, W2{}, K2{});
+      else body(k0, bofs, masked, fl, far, ds, dr, W2{}, K3{});
+    }
+    else if (BIAS && near) body(k0, bofs, masked, fl, far, ds, dr, walk_tag, K2{});
+    else if (decltype(walk_tag)::value == 1 && large) body(k0, bofs, masked, fl, far, ds, dr, std::integral_constant<int, 1>{}, K3{});
+    else if (masked) body(k0, bofs, masked, fl, far, ds, dr, walk_tag, K1{});
     else body(k0, bofs, masked, fl, far, ds, dr, walk_tag, std::integral_constant<int, 0>{});
     if constexpr (decltype(walk_tag)::value == 1) {    // (outside the kinds: accumulators that they all write are copied from one to the other)
 #pragma unroll
@@ -281,12 +321,14 @@ pattn_dq_kernel(const PAttnParams p) {
   }
   {
     const float l = pair_sum(lsum + lsum_lo), d = pair_sum(delta + delta_lo);
-    delta = l > 0.f ? d / l : l == 0.f ? 0.f : l;
-    if (l > 0.f) lse2 += __builtin_log2f(l);
+    delta = sole ? d : l > 0.f ? d / l : l == 0.f ? 0.f : l;
+    if (l > 0.f) ll = __builtin_log2f(l);
+    if (dead || ref == PA_NINF) ref = -PA_NINF;
     if constexpr (FIT) amax = pair_max(amax);
     if (row_ok && h2 == 0) {
       const size_t at = (size_t)unit * p.rows + row;
-      p.st_lse[at] = lse2;
+      p.st_ref[at] = ref;
+      p.st_log[at] = ll;
       p.st_delta[at] = delta;
       if constexpr (FIT) p.st_amax[at] = amax;
     }
@@ -366,7 +408,7 @@ STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256, 2)
 pattn_dkdv_kernel(const PAttnParams p) {
   constexpr int NT = 256, KB = 128, QT = 64;           // keys per workgroup, query rows per tile
   constexpr int SHIFT = __is_same(T, f16) ? 10 : 0;    // P is rounded as 2^SHIFT P
-  constexpr int ROWB = QT * 12 + 16, BUF = 2 * PA_TILE + ROWB;   // Q tile | dO tile | off[64] | -delta[64] | pos[64] | exponent
+  constexpr int ROWB = PA_ROWB, BUF = 2 * PA_TILE + ROWB;        // Q tile | dO tile | off[64] | -delta[64] | pos[64] | ref[64] | log[64] | exponent, large
   char* smem = dyn_smem();                             // two such buffers, then the bias table
   const long long item = pa_item(p);
   if (item >= p.items) return;
@@ -481,13 +523,13 @@ pattn_dkdv_kernel(const PAttnParams p) {
       pa_stage<NT>(gb, smem, d + PA_TILE, tid, wv, [&](int r, int ch) { return at(r, ch, p.lddo); });
     };
     // a row's statistics: loaded by the first wave a tile ahead, written to LDS when the tile's turn comes
-    float x_lse = 0.f, x_delta = 0.f, x_amax = 0.f;
+    float x_ref = 0.f, x_log = 0.f, x_delta = 0.f, x_amax = 0.f;
     auto load_rows = [&](int t) STAR_ALWAYS_INLINE {
       const int r = t * QT + tid;
-      x_lse = -PA_NINF; x_delta = 0.f; x_amax = 0.f;
+      x_ref = -PA_NINF; x_log = 0.f; x_delta = 0.f; x_amax = 0.f;
       if (tid < QT && r < p.rows) {
         const size_t a = (size_t)unit * p.rows + r;
-        x_lse = p.st_lse[a]; x_delta = p.st_delta[a];
+        x_ref = p.st_ref[a]; x_log = p.st_log[a]; x_delta = p.st_delta[a];
         if constexpr (SHIFT) x_amax = p.st_amax[a];
       }
     };
@@ -506,10 +548,13 @@ pattn_dkdv_kernel(const PAttnParams p) {
         const float m = wave_max(x_amax);
         if (m > 0.f) { const int e = pa_fit_exp(m); if (e < e_row) e_row = e; }
       }
-      o[tid] = far - x_lse + (float)SHIFT;
+      const bool large = wave_any(x_ref != -PA_NINF && !(__builtin_fabsf(x_ref) <= PA_LARGE));
+      o[tid] = (far - x_ref) - x_log + (float)SHIFT;
       o[64 + tid] = -x_delta;
       reinterpret_cast<int*>(o)[128 + tid] = rg.qs + pa_row(p, t * QT + tid).i;
-      if (SHIFT && tid == 0) reinterpret_cast<int*>(o)[192] = e_row;
+      o[192 + tid] = x_ref;
+      o[256 + tid] = (float)SHIFT - x_log;
+      if (tid == 0) { reinterpret_cast<int*>(o)[320] = e_row; reinterpret_cast<int*>(o)[321] = large; }
     };
 
     auto tile = [&](int t, int buf) STAR_ALWAYS_INLINE {
@@ -520,7 +565,7 @@ pattn_dkdv_kernel(const PAttnParams p) {
       const float* o = reinterpret_cast<const float*>(smem + bofs + 2 * PA_TILE);
       float pw = 1.f;
       if constexpr (SHIFT) {
-        const int e = wave_uniform(reinterpret_cast<const int*>(o)[192]);
+        const int e = wave_uniform(reinterpret_cast<const int*>(o)[320]);
         if (e != E) {                                    // larger gradients than so far: lower the common exponent
           const float f = pa_pow2(e - E);
 #pragma unroll
@@ -534,7 +579,7 @@ pattn_dkdv_kernel(const PAttnParams p) {
       if (jw >= n || jw > pb + p.right || (jl < pa - p.left && jw >= p.sinks)) return;   // no row of the tile sees a key of the wave
       const bool masked = !(jl < n && jl <= pa + p.right && (jw >= pb - p.left || jl < p.sinks));
       const bool near = BIAS ? !(j0 + KB - 1 - pa <= -p.R || j0 - pb >= p.R) : false;
-      const bool table = BIAS && near, plain = !table && !masked;
+      const bool each = (BIAS && near) || wave_uniform(reinterpret_cast<const int*>(o)[321]), plain = !each && !masked;
 #pragma unroll
       for (int qs = 0; qs < 2; ++qs) {
         f32x16 s, dp;
@@ -556,7 +601,8 @@ pattn_dkdv_kernel(const PAttnParams p) {
           dp = mfma32<T>(g, vf[ks], dp);
         }
         vec<T, 8> pf[2], df[2], pl[2], dl8[2];           // P and dS, sixteen rows each, and what their rounding left
-        // KIND 0: every row sees every key, the bias is one constant (in off); 1: masks; 2: masks, and the bias from the table
+        // KIND 0: every row sees every key, the bias is one constant (in off); 1: masks; 2: masks, the bias from the table (past its ends: the end
+        // values that go on there), and the score rounded as in the forward pass before the row's reference is subtracted
         auto weights = [&](auto kind_tag) STAR_ALWAYS_INLINE {
           constexpr int KIND = decltype(kind_tag)::value;
 #pragma unroll
@@ -570,13 +616,22 @@ pattn_dkdv_kernel(const PAttnParams p) {
               ps = *reinterpret_cast<const vec<int, 4>*>(reinterpret_cast<const int*>(o) + 128 + row);
             }
             // (with a bias a unit is one head: row by row the positions go up by one)
-            const float* tb = KIND == 2 ? tab + (key - (rg.qs + t * QT + row + 3) + p.R + PA_PAD_K) : nullptr;
+            const float* tb = nullptr;
+            f32x4 ref{}, lg{};
+            if constexpr (KIND == 2) {
+              ref = *reinterpret_cast<const f32x4*>(o + 192 + row);
+              lg = *reinterpret_cast<const f32x4*>(o + 256 + row);
+              int at = key - (rg.qs + t * QT + row + 3) + p.R + PA_PAD_K;
+              at = at < 0 ? 0 : at > 2 * p.R + 2 * PA_PAD_K - 3 ? 2 * p.R + 2 * PA_PAD_K - 3 : at;
+              tb = tab + at;
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = 4 * g + e;
-              float add = off[e];
-              if constexpr (KIND == 2) add += tb[3 - e];
-              float pr = fast_exp2(__builtin_fmaf(s[r], p.c, add));
+              float x;
+              if constexpr (KIND == 2) x = (__builtin_fmaf(s[r], p.c, BIAS ? tb[3 - e] : 0.f) - ref[e]) + lg[e];
+              else x = __builtin_fmaf(s[r], p.c, off[e]);
+              float pr = fast_exp2(x);
               const float d0 = KIND == 0 ? dp[r] : dp[r] + dl[e];
               float v = pr * (SHIFT ? d0 * pw : d0);
               if constexpr (KIND != 0) {
@@ -593,7 +648,7 @@ pattn_dkdv_kernel(const PAttnParams p) {
             }
           }
         };
-        if (table) weights(std::integral_constant<int, BIAS ? 2 : 1>{});
+        if (each) weights(std::integral_constant<int, 2>{});
         else if (masked) weights(std::integral_constant<int, 1>{});
         else weights(std::integral_constant<int, 0>{});
 #pragma unroll

@@ -117,3 +117,96 @@ def test_equal_scores_weigh_the_same(backend, dtype, Nq, score, bias, request):
     # the score: 64 products, the scale, the base and back, and log 700 added to it
     total = score + (bias or 0.0)
     within(lse, torch.full((1, 1, Nq), total + 6.551080335).double(), torch.full((1, 1, Nq), 80 * O.U32 * (abs(score) + abs(bias or 0.0))).double(), "lse")
+
+
+SHIFTS = [1500.0, -5000.0, 1e6, -7e6, 1e9, -1e9, 1e30, -1e30]
+
+
+def shifted_backward(ctx, q, k, v, do, H, KH, shift, base, **kw):
+    """gradients with a bias of `base` plus `shift` in every bucket"""
+    dev = ctx.torch_device
+    kw["bias"] = ((base[0] + shift).to(dev), torch.tensor(base[1], dtype=torch.int32, device=dev))
+    a = [t.to(dev) for t in (q, k, v)]
+    out, lse = ctx.pos_attention(*a, H, KH, return_lse=True, **kw)
+    return (out, *ctx.pos_attention_backward(do.to(dev), *a, lse, H, KH, **kw))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shift", SHIFTS)
+def test_one_visible_key_under_a_large_bias(backend, dtype, shift, request):
+    """P is 1 whatever the score: out is V, dV is dO (rounded once; P within 2^-20 of 1), the other gradients are zero"""
+    ctx = ctx_of(backend, dtype, request)
+    q, k, v, do = (randn(n, 1, 200, 128).to(dtype) for n in range(4))
+    out, dq, dk, dv, dt = shifted_backward(ctx, q, k, v, do, 2, 2, shift, (torch.zeros(16, 2), O.bucket_scheme(16, 30, True)), window=(0, 0))
+    assert torch.equal(out.cpu(), v) and not dq.any() and not dk.any() and not dt.any()
+    within(dv, do.double(), (O.half_step(dtype) + 2.0 ** -20) * do.double().abs() + 2.0 ** -25, "dv")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window", [(-1, -1), (70, 0)])
+@pytest.mark.parametrize("shift", SHIFTS)
+def test_many_keys_under_a_large_bias(backend, dtype, window, shift, request):
+    """q is zero, so that a score is the bias alone and a shift of all biases changes nothing: out and gradients are those without it"""
+    ctx = ctx_of(backend, dtype, request)
+    N, H, KH = 300, 2, 1
+    q, k, v, do = torch.zeros(1, N, H * 64), randn(1, 1, N, 64), randn(2, 1, N, 64), randn(3, 1, N, H * 64)
+    q, k, v, do = (t.to(dtype) for t in (q, k, v, do))
+    base = (torch.zeros(16, H), O.bucket_scheme(16, 30, True))
+    ref = O.pos_attention(q, k, v, H, KH, 0.125, *window, bias=base, dout=do, tight=True)
+    got = shifted_backward(ctx, q, k, v, do, H, KH, shift, base, window=window)
+    for n, t in zip(("out", "dq", "dk", "dv", "dtable"), got):
+        within(t, ref[n], ref["tol_" + n], n)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shift", [1500.0, -5000.0])
+def test_scores_beside_a_large_bias(backend, dtype, shift, request):
+    """below and above the size from which scores are rounded one by one (the bounds count the rounding of a score of this size)"""
+    N = 300
+    q, k, v, do = (randn(n, 1, N, 64).to(dtype) for n in range(4))
+    table, buckets = bias_of(True, 1, 9)
+    for window in ((-1, -1), (40, 3)):
+        check_backward(ctx_of(backend, dtype, request), q, k, v, do, 1, 1, window=window, bias=(table + shift, buckets))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [1e5, 1e9])
+def test_one_key_outweighs_the_others(backend, dtype, size, request):
+    """scores of a large size, far apart: P is 1 at the largest and 0 elsewhere.  dV sums the dO of the rows that chose a key, dQ and dK are zero"""
+    ctx = ctx_of(backend, dtype, request)
+    dev = ctx.torch_device
+    N = 150
+    q, k, v, do = (randn(10 + n, 1, N, 64).to(dtype) for n in range(4))
+    s = size / 8 * (q[0].double() @ k[0].double().T)
+    top = s.topk(2, 1).values
+    best = torch.nn.functional.one_hot(s.argmax(1), N).double()
+    # rows whose first two scores are as near as roundings of 64 products are left out of what is compared: they see one key only
+    near = (top[:, 0] - top[:, 1] <= 200 * O.U32 * size / 8 * (q[0].double().abs() @ k[0].double().abs().T).amax(1) + 50)
+    assert int(near.sum()) <= 2
+    do[:, near] = 0
+    a = [t.to(dev) for t in (q, k, v)]
+    out, lse = ctx.pos_attention(*a, 1, scale=size / 8, return_lse=True)
+    dq, dk, dv, _ = ctx.pos_attention_backward(do.to(dev), *a, lse, 1, scale=size / 8)
+    assert torch.equal(out.cpu()[0, ~near], v[0, s.argmax(1)[~near]])
+    assert not dq.any() and not dk.any()
+    g = do[0].double()
+    within(dv[0], best.T @ g, O.half_step(dtype) * (best.T @ g).abs() + (N * O.U32 + 2.0 ** -20) * (best.T @ g.abs()) + 2.0 ** -25, "dv")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("score", [1e6, -1e9])
+def test_gradient_of_equal_large_scores(backend, dtype, score, request):
+    """q and k the same everywhere: each key weighs 1 / N, dV is the mean of dO; dS sums to zero along a row, its parts are (dP - mean dP) / N"""
+    ctx = ctx_of(backend, dtype, request)
+    dev = ctx.torch_device
+    N = 200
+    q, k = torch.ones(1, N, 64).to(dtype), torch.full((1, N, 64), 0.75).to(dtype)
+    v, do = randn(1, 1, N, 64).to(dtype), randn(2, 1, N, 64).to(dtype)
+    a = [t.to(dev) for t in (q, k, v)]
+    bias = (torch.zeros(16, 1, device=dev), ctx.rel_buckets(16, 30))
+    _, lse = ctx.pos_attention(*a, 1, scale=score / 48, bias=bias, return_lse=True)
+    _, _, dv, dt = ctx.pos_attention_backward(do.to(dev), *a, lse, 1, scale=score / 48, bias=bias)
+    zero = torch.zeros(1, N, 64).to(dtype)
+    ref = O.pos_attention(zero, k, v, 1, 1, 0.125, bias=(torch.zeros(16, 1), O.bucket_scheme(16, 30, True)), dout=do, tight=True)
+    within(dv, ref["dv"], ref["tol_dv"], "dv")
+    within(dt, ref["dtable"], ref["tol_dtable"], "dtable")
