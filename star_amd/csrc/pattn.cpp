@@ -133,11 +133,12 @@ static bool pa_grid(PAttnParams& p, long long items, int units, dim3& grid) {
 }
 
 // the backward pass's workspace: row statistics, sums of dS by bucket, parts of dK and dV
-struct PBwdLayout { size_t dsum, part, bytes; };
+struct PBwdLayout { size_t large, dsum, part, bytes; };
 static PBwdLayout pa_bwd_layout(const PAttnArgs& a, const PPlan& q, const PKPlan& k) {
   auto up = [](size_t n) { return (n + 15) & ~(size_t)15; };
   PBwdLayout l;
-  l.dsum = up(4 * (size_t)q.units * q.rows * 4);
+  l.large = up(4 * (size_t)q.units * q.rows * 4);
+  l.dsum = l.large + up((size_t)q.units * q.nblk * 4 * 4);
   l.part = l.dsum + up(a.table ? (size_t)q.units * q.nblk * a.num_buckets * 4 : 0);
   l.bytes = l.part + k.part_slots * 128 * 128 * 4;
   return l;
@@ -240,6 +241,7 @@ int op_pos_attn_bwd(Ctx* ctx, const PAttnArgs& a, float* dtable) {
   const PBwdLayout l = pa_bwd_layout(a, q, kp);
   const size_t st = (size_t)q.units * q.rows;
   p.st_ref = (float*)a.workspace; p.st_log = p.st_ref + st; p.st_delta = p.st_log + st; p.st_amax = p.st_delta + st;
+  p.st_large = (int*)((char*)a.workspace + l.large); p.nlarge = 4 * q.nblk;
   p.dsum = (float*)((char*)a.workspace + l.dsum);
   p.part = (float*)((char*)a.workspace + l.part);
   ProfScope ps(ctx, PK_ATTN_SELF, 0.0, 0.0, a.batch, a.heads, a.Nq, a.Nk);

@@ -56,6 +56,7 @@ struct PAttnParams {
   float* part;                        // nsplit > 1: [unit][split][rows][68]: O[64], m, l
   // backward
   float* st_ref; float* st_log; float* st_delta; float* st_amax;   // [unit][rows]
+  int* st_large; int nlarge;          // [unit][nlarge]: 32 rows with a large reference point among them
   float* dsum;                        // [unit][row block][num_buckets] sums of dS
   int sblk, split_s, split_n;         // dK / dV: the first sblk key blocks (those of the first tokens) in split_s parts each, the others in split_n
 };

@@ -110,6 +110,7 @@ pattn_dq_kernel(const PAttnParams p) {
   const bool dead = !row_ok || lse_in == PA_NINF;      // P = 0
   float ref = dead ? -PA_NINF : lse_in * PA_LOG2E, ll = 0.f;   // P = exp2(y - ref - ll), y the score in base 2
   const bool large = wave_any(!dead && !(__builtin_fabsf(ref) <= PA_LARGE));
+  if (lane == 0) p.st_large[((size_t)unit * p.nblk + qb) * 4 + wv] = large;
   if (large) ref = PA_NINF;                            // (the running maximum)
   const int hi = pa_hi(p, n, pos), lo0 = pa_lo(p, pos), lo = lo0;
   const int lo_c = lo0 < hi ? lo0 : hi;
@@ -216,7 +217,8 @@ pattn_dq_kernel(const PAttnParams p) {
           if constexpr (WALK == 1) x -= ll;
         } else x = __builtin_fmaf(s[kb][r], p.c, off);
         bool see = true;
-        if constexpr (KIND != 0) {
+        if constexpr (WALK == 2) see = s[kb][r] != PA_NINF;
+        else if constexpr (KIND != 0) {
           see = !masked | ((key < hi) & ((key >= lo) | (key < p.sinks)));
           if constexpr (WALK == 1) x = sole ? 0.f : x;
         }
@@ -269,7 +271,8 @@ pattn_dq_kernel(const PAttnParams p) {
       pa_add2(sum_r, low_r, fl ? 0.f : t);
     }
   };
-  auto tile = [&](int it, int buf, auto walk_tag) STAR_ALWAYS_INLINE {
+  auto tile = [&](int it, int buf, auto walk_tag, auto large_tag) STAR_ALWAYS_INLINE {
+    constexpr bool LARGE = decltype(large_tag)::value;
     const int k0 = tile_of(it) * PA_KT, bofs = buf * 2 * PA_TILE;
     if (!pa_sees(p, w, k0)) return;
     const bool masked = !pa_sees_whole(p, w, k0);
@@ -281,18 +284,11 @@ pattn_dq_kernel(const PAttnParams p) {
       far = fl ? far_l : far_r;
     }
     vec<T, 8> ds[4], dr[4];                            // 2^ex dS, sixteen keys each, and what its rounding left
-    using K1 = std::integral_constant<int, 1>;
-    using K2 = std::integral_constant<int, BIAS ? 2 : 3>;
-    using K3 = std::integral_constant<int, 3>;
-    using W2 = std::integral_constant<int, 2>;
-    if (decltype(walk_tag)::value == 0 && large) {
-      if (near) body(k0, bofs, masked, fl, far, ds, dr, W2{}, K2{});
-      else body(k0, bofs, masked, fl, far, ds, dr, W2{}, K3{});
-    }
-    else if (BIAS && near) body(k0, bofs, masked, fl, far, ds, dr, walk_tag, K2{});
-    else if (decltype(walk_tag)::value == 1 && large) body(k0, bofs, masked, fl, far, ds, dr, std::integral_constant<int, 1>{}, K3{});
-    else if (masked) body(k0, bofs, masked, fl, far, ds, dr, walk_tag, K1{});
-    else body(k0, bofs, masked, fl, far, ds, dr, walk_tag, std::integral_constant<int, 0>{});
+    auto with = [&](auto kind_tag) STAR_ALWAYS_INLINE { body(k0, bofs, masked, fl, far, ds, dr, walk_tag, kind_tag); };
+    if (BIAS && near) with(std::integral_constant<int, BIAS ? 2 : 3>{});
+    else if constexpr (LARGE) with(std::integral_constant<int, 3>{});
+    else if (masked) with(std::integral_constant<int, 1>{});
+    else with(std::integral_constant<int, 0>{});
     if constexpr (decltype(walk_tag)::value == 1) {    // (outside the kinds: accumulators that they all write are copied from one to the other)
 #pragma unroll
       for (int u = 0; u < 4; ++u)
@@ -313,13 +309,15 @@ pattn_dq_kernel(const PAttnParams p) {
 
   glds_wait();
   if (total) stage(0, 0);
-  int buf = 0;
-  for (int it = 0; it < total; ++it, buf ^= 1) {
-    glds_wait(); block_sync();
-    stage(it + 1 < total ? it + 1 : 0, buf ^ 1);       // (the second walk's first tile behind the last)
-    tile(it, buf, std::integral_constant<int, 0>{});
-  }
-  {
+  // both walks; a wave with large rows has its own copy of them (with the same barriers), so that the others' code stays as it is without: kinds for
+  // them in one copy cost 13 %
+  auto walks = [&](auto large_tag) STAR_ALWAYS_INLINE {
+    int buf = 0;
+    for (int it = 0; it < total; ++it, buf ^= 1) {
+      glds_wait(); block_sync();
+      stage(it + 1 < total ? it + 1 : 0, buf ^ 1);     // (the second walk's first tile behind the last)
+      tile(it, buf, std::integral_constant<int, decltype(large_tag)::value ? 2 : 0>{}, large_tag);
+    }
     const float l = pair_sum(lsum + lsum_lo), d = pair_sum(delta + delta_lo);
     delta = sole ? d : l > 0.f ? d / l : l == 0.f ? 0.f : l;
     if (l > 0.f) ll = __builtin_log2f(l);
@@ -337,12 +335,14 @@ pattn_dq_kernel(const PAttnParams p) {
       pw = pa_pow2(ex); ipw = pa_pow2(-ex);
       delta *= pw;                                     // (a power of two: dP 2^ex - delta 2^ex is as exact as dP - delta)
     }
-  }
-  for (int it = 0; it < total; ++it, buf ^= 1) {
-    glds_wait(); block_sync();
-    if (it + 1 < total) stage(it + 1, buf ^ 1);
-    tile(it, buf, std::integral_constant<int, 1>{});
-  }
+    for (int it = 0; it < total; ++it, buf ^= 1) {
+      glds_wait(); block_sync();
+      if (it + 1 < total) stage(it + 1, buf ^ 1);
+      tile(it, buf, std::integral_constant<int, 1>{}, large_tag);
+    }
+  };
+  if (__builtin_expect(large, 0)) walks(std::true_type{});
+  else walks(std::false_type{});
   pa_store_row<T>(acc, p.scale * ipw, (T*)p.dQ + (size_t)b * p.bsdq + (size_t)rw.i * p.lddq + (head0 + rw.g) * 64, row_ok);
   if constexpr (BIAS) {
     const float tl2 = wave_sum(sum_l + low_l), tr2 = wave_sum(sum_r + low_r);
@@ -408,7 +408,7 @@ STAR_GLOBAL void STAR_LAUNCH_BOUNDS(256, 2)
 pattn_dkdv_kernel(const PAttnParams p) {
   constexpr int NT = 256, KB = 128, QT = 64;           // keys per workgroup, query rows per tile
   constexpr int SHIFT = __is_same(T, f16) ? 10 : 0;    // P is rounded as 2^SHIFT P
-  constexpr int ROWB = PA_ROWB, BUF = 2 * PA_TILE + ROWB;        // Q tile | dO tile | off[64] | -delta[64] | pos[64] | ref[64] | log[64] | exponent, large
+  constexpr int ROWB = PA_ROWB, BUF = 2 * PA_TILE + ROWB;        // Q tile | dO tile | off[64] | -delta[64] | pos[64] | ref[64] | log[64] | exponent
   char* smem = dyn_smem();                             // two such buffers, then the bias table
   const long long item = pa_item(p);
   if (item >= p.items) return;
@@ -480,7 +480,7 @@ pattn_dkdv_kernel(const PAttnParams p) {
     first = all * sl.part / sl.parts; last = all * (sl.part + 1) / sl.parts;
   }
   long long done = 0;                                  // tiles before the current head's
-  int E = PA_EXP_MAX;                                          // f16: dK is summed as 2^E dK
+  int E = PA_EXP_MAX;                                  // f16: dK is summed as 2^E dK
   for (int w = 0; w < nb * subs; ++w) {
     const int b = shared ? wave_uniform(w / subs) : kb0, sub = shared ? w - b * subs : w;
     const int head0 = kvh * G + sub * p.gp, unit = b * upb + kvh * subs + sub;
@@ -505,6 +505,8 @@ pattn_dkdv_kernel(const PAttnParams p) {
       block_sync();
       far_l = tab[0]; far_r = tab[2 * p.R + 2 * PA_PAD_K];
     } else block_sync();
+    bool large = false;                                  // (no bias) some of the rows are large
+    int reach = p.R;                                     // where the bias is one constant
 
     auto bounds = [&](int t, int& pa, int& pb) STAR_ALWAYS_INLINE {    // positions of a tile's first and last row
       const int rl = t * QT + QT - 1 < p.rows - 1 ? t * QT + QT - 1 : p.rows - 1;
@@ -548,13 +550,12 @@ pattn_dkdv_kernel(const PAttnParams p) {
         const float m = wave_max(x_amax);
         if (m > 0.f) { const int e = pa_fit_exp(m); if (e < e_row) e_row = e; }
       }
-      const bool large = wave_any(x_ref != -PA_NINF && !(__builtin_fabsf(x_ref) <= PA_LARGE));
       o[tid] = (far - x_ref) - x_log + (float)SHIFT;
       o[64 + tid] = -x_delta;
       reinterpret_cast<int*>(o)[128 + tid] = rg.qs + pa_row(p, t * QT + tid).i;
       o[192 + tid] = x_ref;
       o[256 + tid] = (float)SHIFT - x_log;
-      if (tid == 0) { reinterpret_cast<int*>(o)[320] = e_row; reinterpret_cast<int*>(o)[321] = large; }
+      if (SHIFT && tid == 0) reinterpret_cast<int*>(o)[320] = e_row;
     };
 
     auto tile = [&](int t, int buf) STAR_ALWAYS_INLINE {
@@ -578,8 +579,8 @@ pattn_dkdv_kernel(const PAttnParams p) {
       }
       if (jw >= n || jw > pb + p.right || (jl < pa - p.left && jw >= p.sinks)) return;   // no row of the tile sees a key of the wave
       const bool masked = !(jl < n && jl <= pa + p.right && (jw >= pb - p.left || jl < p.sinks));
-      const bool near = BIAS ? !(j0 + KB - 1 - pa <= -p.R || j0 - pb >= p.R) : false;
-      const bool each = (BIAS && near) || wave_uniform(reinterpret_cast<const int*>(o)[321]), plain = !each && !masked;
+      const bool near = BIAS ? !(j0 + KB - 1 - pa <= -reach || j0 - pb >= reach) : false;
+      const bool table = BIAS && near, plain = !table && !masked && !large;
 #pragma unroll
       for (int qs = 0; qs < 2; ++qs) {
         f32x16 s, dp;
@@ -601,14 +602,17 @@ pattn_dkdv_kernel(const PAttnParams p) {
           dp = mfma32<T>(g, vf[ks], dp);
         }
         vec<T, 8> pf[2], df[2], pl[2], dl8[2];           // P and dS, sixteen rows each, and what their rounding left
-        // KIND 0: every row sees every key, the bias is one constant (in off); 1: masks; 2: masks, the bias from the table (past its ends: the end
-        // values that go on there), and the score rounded as in the forward pass before the row's reference is subtracted
+        // KIND 0: every row sees every key, the bias is one constant (in off); 1: masks; 2: masks, and the bias from the table (past its ends too: the
+        // end values go on there); 3: large rows without a bias, masks.  2 and 3 (EACH) round the score as the forward pass does before the row's
+        // reference is subtracted
         auto weights = [&](auto kind_tag) STAR_ALWAYS_INLINE {
           constexpr int KIND = decltype(kind_tag)::value;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {                  // rows 8 g + 4 h2 + (0 .. 3) of the 32
             const int row = qs * 32 + 8 * g + 4 * h2;
-            const f32x4 off = *reinterpret_cast<const f32x4*>(o + row);
+            constexpr bool EACH = KIND == (BIAS ? 2 : 3);
+            f32x4 off{};
+            if constexpr (!EACH) off = *reinterpret_cast<const f32x4*>(o + row);
             vec<int, 4> ps{};
             f32x4 dl{};
             if constexpr (KIND != 0) {
@@ -618,7 +622,7 @@ pattn_dkdv_kernel(const PAttnParams p) {
             // (with a bias a unit is one head: row by row the positions go up by one)
             const float* tb = nullptr;
             f32x4 ref{}, lg{};
-            if constexpr (KIND == 2) {
+            if constexpr (EACH) {
               ref = *reinterpret_cast<const f32x4*>(o + 192 + row);
               lg = *reinterpret_cast<const f32x4*>(o + 256 + row);
               int at = key - (rg.qs + t * QT + row + 3) + p.R + PA_PAD_K;
@@ -629,7 +633,7 @@ pattn_dkdv_kernel(const PAttnParams p) {
             for (int e = 0; e < 4; ++e) {
               const int r = 4 * g + e;
               float x;
-              if constexpr (KIND == 2) x = (__builtin_fmaf(s[r], p.c, BIAS ? tb[3 - e] : 0.f) - ref[e]) + lg[e];
+              if constexpr (EACH) x = (__builtin_fmaf(s[r], p.c, BIAS ? tb[3 - e] : 0.f) - ref[e]) + lg[e];
               else x = __builtin_fmaf(s[r], p.c, off[e]);
               float pr = fast_exp2(x);
               const float d0 = KIND == 0 ? dp[r] : dp[r] + dl[e];
@@ -648,7 +652,8 @@ pattn_dkdv_kernel(const PAttnParams p) {
             }
           }
         };
-        if (each) weights(std::integral_constant<int, 2>{});
+        if (table) weights(std::integral_constant<int, BIAS ? 2 : 1>{});
+        else if (!BIAS && large) weights(std::integral_constant<int, BIAS ? 1 : 3>{});
         else if (masked) weights(std::integral_constant<int, 1>{});
         else weights(std::integral_constant<int, 0>{});
 #pragma unroll
@@ -673,8 +678,13 @@ pattn_dkdv_kernel(const PAttnParams p) {
       }
     };
 
+    int some = 0;                                        // of the tiles' rows, 32 to a word
+    for (int i = 2 * t0 + lane; i < 2 * t1; i += 64) some |= p.st_large[(size_t)unit * p.nlarge + i];
     load_rows(t0);
     glds_wait();                                         // no compiler-visible load in flight beside the hand-written DMA's first use
+    // with a large row among them all tiles take the kind that rounds the scores one by one; with a bias as if all were near.  (This costs the others
+    // 2 % of this kernel; a kind of its own with a bias, too, or a flag per tile 4 - 5 %)
+    if (wave_any(some)) { if (BIAS) reach = 1 << 30; else large = true; }
     stage(t0, 0);
     for (int t = t0; t < t1; ++t) {
       const int buf = (t - t0) & 1;
