@@ -197,6 +197,8 @@ int star_layer_norm_bwd(star_ctx* ctx, const void* dy, int64_t lddy, const void*
  * [0, Nk] and buckets outside [0, num_buckets) are clamped to it, q_start to +-2^29.  K and V rows that no query row of a 128-row block
  * (256 for long inputs) sees are not read; a NaN or an infinity in a V row (backward: also K, Q, dO rows) may reach the other rows of the
  * block that the row belongs to.  Sums are fp32; probabilities (and dS) are rounded to the 16-bit type for the second product.
+ * Biases beyond +-2.36e38 (where base 2 ends) count as fp32's lowest or highest value: beside any other such keys weigh nothing, or all; a row that sees no
+ * others averages them, its lse is that value.  Scores are fp32 sums: what a large bias rounds away from them is lost in both passes alike.
  * Outputs overlap neither each other nor an input (strided views of one buffer, a fused projection's, are fine).
  * The backward pass takes lse from the forward pass; gradients of heads, or of K and V, that are shared are sums over what shares them. */
 typedef struct star_pos_attn_desc {

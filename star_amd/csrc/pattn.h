@@ -106,13 +106,19 @@ STAR_DEV long long pa_item(const PAttnParams& p) {
 
 // The bias of one head by relative position, times log2(e), in LDS: tab[i] belongs to j - p = i - R - PAD.  The end values go on for PAD
 // entries either way, so that in a tile that reaches into (-R, R) every score's entry is at a fixed distance from its lane's first: no
-// clamping per score.  The type's lowest value stays finite
+// clamping per score.  The type's lowest and highest values stay finite: whatever leaves the range in base 2 (beyond +-2.36e38) is held at
+// +-3.40e38, the log-sum-exp of a row that sees nothing better is the type's lowest (highest) value
+constexpr float PA_MOST = 3.4028235e38f;
 constexpr int PA_PAD = 128, PA_PAD_Q = 96, PA_PAD_K = 192;     // a wave's 64 rows against 64 keys; dQ: 32 rows; dK / dV: 64 rows against 128 keys
 STAR_DEV float pa_bias_at(const PAttnParams& p, int head, int k) {       // of bucket k
   k = k < 0 ? 0 : k >= p.num_buckets ? p.num_buckets - 1 : k;
   const float v = p.table[(size_t)k * p.heads + head];
   const float w = v * PA_LOG2E;
-  return w == PA_NINF && v != PA_NINF ? -3.4028235e38f : w;
+  return __builtin_fabsf(w) > PA_MOST && __builtin_fabsf(v) <= PA_MOST ? __builtin_copysignf(PA_MOST, v) : w;
+}
+// log sum exp in base e from the maximum and the sum relative to it
+STAR_DEV float pa_lse(float m, float l) {
+  return l == 0.f ? PA_NINF : __builtin_fabsf(m) == PA_MOST ? m : (m + __builtin_log2f(l)) * PA_LN2;
 }
 template <int NT, int PAD>
 STAR_DEV void pa_bias_table(const PAttnParams& p, int head, float* tab) {
@@ -453,7 +459,7 @@ pattn_fwd_kernel(const PAttnParams p) {
     } else {
       pa_store_row<T>(oacc[qi], l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l, (T*)p.O + (size_t)b * p.bso + (size_t)rw.i * p.ldo + (head0 + rw.g) * 64, ok);
       if (p.lse && ok && h2 == 0)
-        p.lse[((size_t)b * p.heads + head0 + rw.g) * p.Nq + rw.i] = l == 0.f ? PA_NINF : (m_run[qi] + __builtin_log2f(l)) * PA_LN2;
+        p.lse[((size_t)b * p.heads + head0 + rw.g) * p.Nq + rw.i] = pa_lse(m_run[qi], l);
     }
   }
 }
@@ -500,7 +506,7 @@ pattn_combine_kernel(const PAttnParams p) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) out[e] = from_f32<T>(o[e] * mul);
   *reinterpret_cast<vec<T, 4>*>((T*)p.O + (size_t)b * p.bso + (size_t)rw.i * p.ldo + head * 64 + 4 * sub) = out;
-  if (p.lse && sub == 0) p.lse[((size_t)b * p.heads + head) * p.Nq + rw.i] = l == 0.f ? PA_NINF : (m + __builtin_log2f(l)) * PA_LN2;
+  if (p.lse && sub == 0) p.lse[((size_t)b * p.heads + head) * p.Nq + rw.i] = pa_lse(m, l);
 }
 
 }  // namespace star

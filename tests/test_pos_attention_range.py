@@ -210,3 +210,55 @@ def test_gradient_of_equal_large_scores(backend, dtype, score, request):
     ref = O.pos_attention(zero, k, v, 1, 1, 0.125, bias=(torch.zeros(16, 1), O.bucket_scheme(16, 30, True)), dout=do, tight=True)
     within(dv, ref["dv"], ref["tol_dv"], "dv")
     within(dt, ref["dtable"], ref["tol_dtable"], "dtable")
+
+
+MOST = torch.finfo(torch.float32).max
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Nq", [1, 200])
+@pytest.mark.parametrize("shift", [-MOST, MOST, -2.5e38])
+def test_every_bias_at_the_end_of_the_range(backend, dtype, Nq, shift, request):
+    """all keys weigh the same, their scores lost beside the bias; with q = 0 the gradients are those without a bias"""
+    ctx = ctx_of(backend, dtype, request)
+    q, k, v, do = torch.zeros(1, Nq, 64), randn(1, 1, 200, 64), randn(2, 1, 200, 64), randn(3, 1, Nq, 64)
+    q, k, v, do = (t.to(dtype) for t in (q, k, v, do))
+    base = (torch.zeros(16, 1), O.bucket_scheme(16, 30, True))
+    ref = O.pos_attention(q, k, v, 1, 1, 0.125, bias=base, dout=do, tight=True)
+    got = shifted_backward(ctx, q, k, v, do, 1, 1, shift, base)
+    for n, t in zip(("out", "dq", "dk", "dv", "dtable"), got):
+        within(t, ref[n], ref["tol_" + n], n)
+    dev = ctx.torch_device
+    bias = (torch.full((16, 1), shift, device=dev), torch.tensor(base[1], dtype=torch.int32, device=dev))
+    out, lse = ctx.pos_attention(randn(4, 1, Nq, 64).to(dtype).to(dev), k.to(dev), v.to(dev), 1, bias=bias, return_lse=True)
+    within(out, ref["out"], ref["tol_out"], "out")
+    if abs(shift) == MOST:
+        assert bool((lse == shift).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("which", ["lowest", "highest", "both"])
+def test_some_biases_at_the_end_of_the_range(backend, dtype, which, request):
+    """buckets at the lowest value hide their keys from rows that see others, as -inf does; buckets at the highest hide all others"""
+    ctx = ctx_of(backend, dtype, request)
+    dev = ctx.torch_device
+    N = 150
+    q, k, v, do = (randn(20 + n, 1, N, 64).to(dtype) for n in range(4))
+    q = q * (which == "lowest")                               # (a highest bias loses the scores beside it)
+    table, buckets = bias_of(True, 1, 9)
+    hidden = table.clone()
+    if which != "highest":
+        table[3], hidden[3] = -MOST, -float("inf")
+    if which != "lowest":
+        table[0], hidden = MOST, torch.full_like(hidden, -float("inf"))
+        hidden[0] = 0.0
+    want = O.pos_attention(q, k, v, 1, 1, 0.125, bias=(hidden, buckets), dout=do, tight=True)
+    assert torch.isfinite(want["lse"]).all()
+    kw = dict(bias=(table.to(dev), torch.tensor(buckets, dtype=torch.int32, device=dev)))
+    a = [t.to(dev) for t in (q, k, v)]
+    out, lse = ctx.pos_attention(*a, 1, return_lse=True, **kw)
+    got = ctx.pos_attention_backward(do.to(dev), *a, lse, 1, **kw)
+    for n, t in zip(("out", "dq", "dk", "dv", "dtable"), (out, *got)):
+        within(t, want[n], want["tol_" + n], n)
+    if which != "lowest":
+        assert bool((lse == MOST).all())
