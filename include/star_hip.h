@@ -224,7 +224,7 @@ typedef struct star_pos_attn_grads {
 } star_pos_attn_grads;
 size_t star_pos_attn_workspace(star_ctx* ctx, const star_pos_attn_desc* d, int32_t backward);
 int star_pos_attn_fwd(star_ctx* ctx, const star_pos_attn_desc* d);
-/* d as in the forward pass (O is not read); every element of dQ, dK, dV and dbias_table is written.  No atomics on floats in memory: the same
+/* d as in the forward pass (O is not read); every element of dQ, dK, dV (none where batch is 0) and dbias_table is written.  No atomics on floats in memory: the same
  * call gives the same bits. */
 int star_pos_attn_bwd(star_ctx* ctx, const star_pos_attn_desc* d, const star_pos_attn_grads* g);
 /* The buckets of relative positions j - p = -max_distance .. max_distance (host int32 [2 * max_distance + 1]) in the scheme of text encoders

@@ -679,6 +679,8 @@ class Context:
         dtable = torch.empty(d.num_buckets, heads, dtype=torch.float32, device=self.torch_device) if bias is not None else None
         g.dbias_table = dtable.data_ptr() if dtable is not None else None
         ws = self._pos_workspace(d, True)
+        if B == 0:                              # (no sequence: the C entry writes only the table's gradient, keys shared by none have zeros)
+            dk.zero_(), dv.zero_()
         self._launch(self.lib.pos_attn_bwd, "pos_attn_bwd", ctypes.byref(d), ctypes.byref(g))
         del ws
         return dq, dk, dv, dtable
