@@ -90,6 +90,8 @@ int op_layer_norm_train(Ctx* ctx, const void* x, long long ldx, void* y, long lo
   ProfScope ps(ctx, PK_LN, 0.0, 4.0 * rows * (double)C);
   const bool v = !((C | ldx | ldy) & 7) && al16(x) && al16(y) && al16(gamma) && al16(beta);
   const LnShape sh = ln_shape(C, v, false);
+  const long long rpb = sh.lpr ? 4 * (64 / sh.lpr) : 1;   // (a launch counts its threads in 32 bits)
+  if ((rows + rpb - 1) / rpb * 256 > 0xffffffffLL) return ctx->fail("layer_norm_train: too many rows for this width");
   LnTrainParams p{x, nullptr, y, gamma, beta, stats, nullptr, ldx, 0, ldy, rows, C, sh.lpr, ln_streams(rows, C), eps};
   if (ctx->dtype == DT_F16) v ? ln_go<f16, true>(ctx, p, sh.cpl, -1) : ln_go<f16, false>(ctx, p, sh.cpl, -1);
   else v ? ln_go<bf16, true>(ctx, p, sh.cpl, -1) : ln_go<bf16, false>(ctx, p, sh.cpl, -1);

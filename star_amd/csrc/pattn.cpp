@@ -123,11 +123,12 @@ static PAttnParams pa_params(const PAttnArgs& a, const PPlan& q) {
 }
 
 // items to workgroups: contiguous runs per XCD where there are units enough for each (its L2 keeps the unit's K and V), else one after the other
-static bool pa_grid(PAttnParams& p, long long items, int units, dim3& grid) {
+// (false: more threads than the 32 bits that a launch counts them in)
+static bool pa_grid(PAttnParams& p, long long items, int units, int threads, dim3& grid) {
   p.items = items;
   p.swz = units >= 8 ? 1 : 0;
   const long long g = p.swz ? 8 * ((items + 7) / 8) : items;
-  if (g > 0x7fffffffLL) return false;
+  if (g * threads > 0xffffffffLL) return false;
   grid = dim3((unsigned)g);
   return true;
 }
@@ -178,7 +179,7 @@ int op_pos_attn_fwd(Ctx* ctx, const PAttnArgs& a) {
     return ctx->fail("pos_attn_fwd: workspace missing, too small (star_pos_attn_workspace) or not 16-byte aligned");
   p.part = (float*)a.workspace;
   dim3 grid;
-  if (!pa_grid(p, (long long)q.units * q.nblk * q.nsplit, q.units, grid)) return ctx->fail("pos_attn_fwd: too many workgroups");
+  if (!pa_grid(p, (long long)q.units * q.nblk * q.nsplit, q.units, 64 * q.nw, grid)) return ctx->fail("pos_attn_fwd: too many workgroups");
   ProfScope ps(ctx, PK_ATTN_SELF, 0.0, 0.0, a.batch, a.heads, a.Nq, a.Nk);
   if (ctx->dtype == DT_F16) return a.table ? fwd_t<f16, 1>(ctx, p, q, grid) : fwd_t<f16, 0>(ctx, p, q, grid);
   return a.table ? fwd_t<bf16, 1>(ctx, p, q, grid) : fwd_t<bf16, 0>(ctx, p, q, grid);
@@ -189,14 +190,14 @@ static int bwd_t(Ctx* ctx, PAttnParams p, const PPlan& q, const PKPlan& kp, floa
   const int R2 = 2 * p.R + 1;
   dim3 grid;
   if (p.batch > 0 && p.Nq > 0) {
-    if (!pa_grid(p, (long long)q.units * q.nblk, q.units, grid)) return ctx->fail("pos_attn_bwd: too many workgroups");
+    pa_grid(p, (long long)q.units * q.nblk, q.units, 256, grid);
     const size_t smem = 4 * PA_TILE + (BIAS ? (size_t)(5 * (R2 + 2 * PA_PAD_Q) + 64 * PA_SKEW + 16) * 4 : 0);
     STAR_LAUNCH((pattn_dq_kernel<T, BIAS, COMP>), grid, dim3(256), smem, ctx->stream, p);
   }
   if (p.batch > 0 && p.Nk > 0) {
     PAttnParams k = p;
     k.nblk = kp.slots; k.sblk = kp.sblk; k.split_s = kp.split_s; k.split_n = kp.split_n;
-    if (!pa_grid(k, (long long)kp.units * kp.slots, kp.units, grid)) return ctx->fail("pos_attn_bwd: too many workgroups");
+    pa_grid(k, (long long)kp.units * kp.slots, kp.units, 256, grid);
     const size_t smem = 2 * (2 * PA_TILE + PA_ROWB) + (BIAS ? (size_t)(R2 + 2 * PA_PAD_K) * 4 : 0);
     STAR_LAUNCH((pattn_dkdv_kernel<T, BIAS, COMP>), grid, dim3(256), smem, ctx->stream, k);
     if (kp.part_slots) {
@@ -238,6 +239,9 @@ int op_pos_attn_bwd(Ctx* ctx, const PAttnArgs& a, float* dtable) {
   if (need && (!a.workspace || a.workspace_bytes < need || !al16(a.workspace)))
     return ctx->fail("pos_attn_bwd: workspace missing, too small (star_pos_attn_workspace) or not 16-byte aligned");
   const PKPlan kp = pa_kplan(ctx, a, q);
+  dim3 grid;                                             // (before the first launch: nothing is left half done)
+  if (!pa_grid(p, (long long)q.units * q.nblk, q.units, 256, grid) || !pa_grid(p, (long long)kp.units * kp.slots, kp.units, 256, grid))
+    return ctx->fail("pos_attn_bwd: too many workgroups");
   const PBwdLayout l = pa_bwd_layout(a, q, kp);
   const size_t st = (size_t)q.units * q.rows;
   p.st_ref = (float*)a.workspace; p.st_log = p.st_ref + st; p.st_delta = p.st_log + st; p.st_amax = p.st_delta + st;

@@ -34,3 +34,35 @@ def test_no_sequence_over_shared_keys(backend, request):
     dq, dk, dv, dt = ctx.pos_attention_backward(out, q, kv, kv, lse, 2, bias=bias, dk=given[0], dv=given[1])
     assert dq.shape == (0, 3, 128) and dk.shape == dv.shape == kv.shape
     assert not given.any() and not dt.any()
+
+
+def test_launches_past_what_a_grid_holds_are_refused(backend, request):
+    """2^24 workgroups of 256 threads, or 2^26 of 64, are more threads than a launch counts: refused on the host, before anything runs"""
+    ctx = ctx_of(backend, torch.float16, request)
+    dev = ctx.torch_device
+    t = torch.zeros(2, 64, dtype=torch.float16, device=dev)
+    f = torch.zeros(64, dtype=torch.float32, device=dev)
+
+    def call(batch, Nq, backward):
+        d = L.PosAttnDesc()
+        d.Q = d.K = d.V = t.data_ptr()
+        d.O, d.lse = t[1:].data_ptr(), f.data_ptr()
+        d.ldq = d.ldk = d.ldv = d.ldo = 64
+        d.bsq, d.bsk, d.bsv, d.bso = 64 * Nq, 0, 0, 64 * Nq
+        d.Nq, d.Nk, d.heads, d.kv_heads, d.batch, d.scale, d.left, d.right = Nq, 1, 1, 1, batch, 1.0, -1, -1
+        need = ctx.lib.pos_attn_workspace(ctx.h, ctypes.byref(d), backward)
+        d.workspace, d.workspace_bytes = f.data_ptr(), need      # (as if there were so much: nothing is launched)
+        if not backward:
+            return ctx.lib.pos_attn_fwd(ctx.h, ctypes.byref(d))
+        g = L.PosAttnGrads()
+        o = torch.zeros(3, 64, dtype=torch.float16, device=dev)
+        g.dO, g.dQ, g.dK, g.dV = t[1:].data_ptr(), *(x.data_ptr() for x in o)
+        g.lddo = g.lddq = g.lddk = g.lddv = 64
+        g.bsdo, g.bsdq, g.bsdk, g.bsdv = 64 * Nq, 64 * Nq, 0, 0
+        return ctx.lib.pos_attn_bwd(ctx.h, ctypes.byref(d), ctypes.byref(g))
+
+    for batch, Nq, backward in ((1 << 26, 1, 0), (1 << 24, 33, 0), (1 << 24, 1, 1)):
+        assert call(batch, Nq, backward) and b"too many workgroups" in ctx.lib.last_error(ctx.h), (batch, Nq, backward)
+    x = t.data_ptr()
+    for rows, C in ((1 << 24, 2561), (1 << 26, 2560), (1 << 26, 1304), (1 << 26, 512)):
+        assert ctx.lib.layer_norm_train(ctx.h, x, C, x, C, None, None, None, rows, C, 1e-5) and b"too many rows" in ctx.lib.last_error(ctx.h), (rows, C)
