@@ -66,3 +66,27 @@ def test_launches_past_what_a_grid_holds_are_refused(backend, request):
     x = t.data_ptr()
     for rows, C in ((1 << 24, 2561), (1 << 26, 2560), (1 << 26, 1304), (1 << 26, 512)):
         assert ctx.lib.layer_norm_train(ctx.h, x, C, x, C, None, None, None, rows, C, 1e-5) and b"too many rows" in ctx.lib.last_error(ctx.h), (rows, C)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_all_gradients_of_a_cache_past_32_bits(dtype):
+    """the last keys of a cache of more than 2^32 bytes are the ones that count: dv of them too, with a bias and without"""
+    ctx = L.Context(0, dtype)
+    Nk, tail, Nq = (1 << 32) // (2 * 1024) + 300, 500, 70
+    k = torch.zeros(1, Nk, 1024, dtype=dtype, device="cuda")[:, :, 960:]
+    v = torch.zeros(1, Nk, 1024, dtype=dtype, device="cuda")[:, :, :64]
+    g = torch.Generator().manual_seed(3)
+    k[:, -tail:], v[:, -tail:] = (torch.randn(1, tail, 64, generator=g).to(dtype).cuda() for _ in range(2))
+    q, do = (torch.randn(1, Nq, 64, generator=g).to(dtype) for _ in range(2))
+    for bias in (None, (torch.randn(16, 1, generator=g), O.bucket_scheme(16, 30, True))):
+        ref = O.pos_attention(q, k[:, -tail:].cpu(), v[:, -tail:].cpu(), 1, 1, 0.125, 200, 0, 0, bias=bias, dout=do, tight=True)
+        kw = {"window": (200, 0)}
+        if bias is not None:
+            kw["bias"] = (bias[0].cuda(), torch.tensor(bias[1], dtype=torch.int32, device="cuda"))
+        out, lse = ctx.pos_attention(q.cuda(), k, v, 1, return_lse=True, **kw)
+        dq, dk, dv, dt = ctx.pos_attention_backward(do.cuda(), q.cuda(), k, v, lse, 1, **kw)
+        for n, t in (("out", out), ("dq", dq), ("dk", dk[:, -tail:]), ("dv", dv[:, -tail:]), ("dtable", dt)):
+            if t is not None:
+                assert (t.cpu().double() - ref[n]).abs().le(ref["tol_" + n]).all(), n
+        assert not dk[:, :-tail].any() and not dv[:, :-tail].any()
