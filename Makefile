@@ -10,7 +10,8 @@ HIP_OBJS := $(patsubst $(CSRC)/%.cpp,build/hip/%.o,$(SRCS))
 EMU_OBJS := $(patsubst $(CSRC)/%.cpp,build/emu/%.o,$(SRCS)) build/emu/hostemu.o
 # no packed fp32 instructions (v_pk_add / mul / fma_f32): hipcc forms them from ordinary float code, and some of their forms have given
 # wrong results on this hardware now and then, with no error (the host pass warns that it does not know the feature: harmless)
-HIPFLAGS := --offload-arch=gfx950 -O3 -std=c++17 -fPIC -x hip -Wno-unused-value -Wno-inline-asm -ffp-contract=fast -Xclang -target-feature -Xclang -packed-fp32-ops
+NO_PK_FP32 := -Xclang -target-feature -Xclang -packed-fp32-ops
+HIPFLAGS := --offload-arch=gfx950 -O3 -std=c++17 -fPIC -x hip -Wno-unused-value -Wno-inline-asm -ffp-contract=fast $(NO_PK_FP32)
 EMUFLAGS := -O2 -g -std=c++17 -fPIC -DSTAR_HOSTEMU=1 -DSTAR_BENCH_VARIANTS=1 -mavx2 -mf16c -mfma -Wno-unused-value -Wno-psabi -Wno-psabi
 
 all: hip emu
@@ -62,9 +63,9 @@ tools/bench/libstar_hip_bench.so: $(BENCH_OBJS)
 # torch-free timing harness over the C ABI (dlopen()s a build of the library): seconds instead of minutes per A/B on a fresh GPU box
 cbench: tools/cbench/cbench tools/cbench/cbench_emu tools/probe/mfma_valu_overlap
 tools/probe/mfma_valu_overlap: tools/probe/mfma_valu_overlap.hip
-	$(HIPCC) -O2 --offload-arch=gfx950 $< -o $@
+	$(HIPCC) -O2 --offload-arch=gfx950 $(NO_PK_FP32) $< -o $@
 tools/cbench/cbench: tools/cbench/cbench.cpp include/star_hip.h
-	$(HIPCC) -O2 --offload-arch=gfx950 $< -o $@ -ldl
+	$(HIPCC) -O2 --offload-arch=gfx950 $(NO_PK_FP32) $< -o $@ -ldl
 tools/cbench/cbench_emu: tools/cbench/cbench.cpp include/star_hip.h
 	$(CXX) -O2 -DCBENCH_EMU $< -o $@ -ldl
 

@@ -2,7 +2,7 @@
 // buffers with N(0,1)-like 16-bit operands and times kernel launches with HIP events on the context's stream.  A fresh GPU box
 // spends 1-2 minutes paging in `import torch`; this binary starts in a second, so a kernel A/B costs seconds of the GPU budget.
 //
-//   hipcc -O2 --offload-arch=gfx950 tools/cbench/cbench.cpp -o tools/cbench/cbench -ldl          (the GPU build)
+//   hipcc -O2 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/cbench/cbench.cpp -o tools/cbench/cbench -ldl          (the GPU build)
 //   g++ -O2 -DCBENCH_EMU tools/cbench/cbench.cpp -o tools/cbench/cbench_emu -ldl                 (against libstar_emu.so: plumbing check)
 //   cbench <lib.so> <f16|bf16> <spec file | -> [reps]
 // spec lines (# comments):

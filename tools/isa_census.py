@@ -19,7 +19,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 def main():
     src, pat = sys.argv[1], sys.argv[2]
     bench = "--bench" in sys.argv
-    flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-x", "hip", "-Wno-unused-value", "-Wno-inline-asm", "-ffp-contract=fast",
+    flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-x", "hip", "-Wno-unused-value", "-Wno-inline-asm", "-ffp-contract=fast", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
              "-I" + os.path.join(ROOT, "include"), "--cuda-device-only", "-S"]
     if src.startswith("attn"):
         flags += ["-fno-honor-nans", "-fno-slp-vectorize"]

@@ -2,8 +2,9 @@
 // One workgroup of 4 waves (one per SIMD, a single CU: no power throttling) loops over {1 MFMA 32x32x16 f16, NV independent VALU
 // instructions} x 4 accumulators; time per MFMA slot against NV says whether the VALU issues ride in the MFMA's 8 passes (flat up to
 // ~7 x 4-cycle issues) or serialise behind it (linear from NV = 1).  Accumulators in AGPRs ("a" form) or architectural VGPRs ("v" form,
-// what -mllvm -amdgpu-mfma-vgpr-form produces for gemm_as.h / gemm_tq.h); VALU = v_fma_f32, v_pk_fma_f32 or v_exp_f32.
-//   hipcc -O2 --offload-arch=gfx950 tools/probe/mfma_valu_overlap.hip -o tools/probe/mfma_valu_overlap && tools/probe/mfma_valu_overlap
+// what -mllvm -amdgpu-mfma-vgpr-form produces for gemm_as.h / gemm_tq.h); VALU = v_fma_f32, v_exp_f32 and others.
+// (Packed fp32 is not among them: some forms of it have given wrong results on this hardware, nothing here is built with it.)
+//   hipcc -O2 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/probe/mfma_valu_overlap.hip -o tools/probe/mfma_valu_overlap && tools/probe/mfma_valu_overlap
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>
@@ -19,14 +20,12 @@ template <int FORM> __device__ __forceinline__ void mfma(f32x16& acc, f16x8 a, f
   else if constexpr (FORM == 1) asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(acc) : "v"(a), "v"(b));
   else asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(acc) : "v"(a), "a"(b));   // FORM 2: gemm_as.h's form -- B operand (the A panel) from an AGPR, accumulator in VGPRs
 }
-// KIND: 0 v_fma_f32, 1 v_pk_fma_f32, 2 v_exp_f32, 3 v_pk_add_f16, 4 v_pk_mul_f32, 5 v_cvt_pk_f16_f32 (e64), 6 v_max3_f32, 7 ds_read_b128
+// KIND: 0 v_fma_f32, 2 v_exp_f32, 3 v_pk_add_f16, 5 v_cvt_pk_f16_f32 (e64), 6 v_max3_f32, 7 ds_read_b128
 // (LDS), 8 v_accvgpr_read_b32, 9 v_permlane32_swap
 template <int KIND> __device__ __forceinline__ void valu(float& x, f32x2& p, float y, float z, const char* lds, f32x16& spare) {
   if constexpr (KIND == 0) asm volatile("v_fma_f32 %0, %0, %1, %2" : "+v"(x) : "v"(y), "v"(z));
-  else if constexpr (KIND == 1) asm volatile("v_pk_fma_f32 %0, %0, %1, %1" : "+v"(p) : "v"(p));
   else if constexpr (KIND == 2) asm volatile("v_exp_f32 %0, %0" : "+v"(x));
   else if constexpr (KIND == 3) asm volatile("v_pk_add_f16 %0, %0, %1" : "+v"(x) : "v"(y));
-  else if constexpr (KIND == 4) asm volatile("v_pk_mul_f32 %0, %0, %1" : "+v"(p) : "v"(p));
   else if constexpr (KIND == 5) asm volatile("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(x) : "v"(y), "v"(z));
   else if constexpr (KIND == 6) asm volatile("v_max3_f32 %0, %0, %1, %2" : "+v"(x) : "v"(y), "v"(z));
   else if constexpr (KIND == 7) {
@@ -121,8 +120,6 @@ int main(int argc, char** argv) {
     for (int nb : {1, 256}) {
       sweep<0, 0>(out, iters, nb, "accumulators in AGPRs, VALU = v_fma_f32");
       sweep<1, 0>(out, iters, nb, "accumulators in VGPRs, VALU = v_fma_f32");
-      sweep<0, 1>(out, iters, nb, "accumulators in AGPRs, VALU = v_pk_fma_f32");
-      sweep<1, 1>(out, iters, nb, "accumulators in VGPRs, VALU = v_pk_fma_f32");
       sweep<0, 2>(out, iters, nb, "accumulators in AGPRs, VALU = v_exp_f32");
       sweep<1, 2>(out, iters, nb, "accumulators in VGPRs, VALU = v_exp_f32");
     }
@@ -130,7 +127,6 @@ int main(int argc, char** argv) {
   }
   // one workgroup (boost clock), accumulators in AGPRs: the other instruction kinds a K / key loop carries
   sweep<0, 3>(out, iters, 1, "v_pk_add_f16");
-  sweep<0, 4>(out, iters, 1, "v_pk_mul_f32");
   sweep<0, 5>(out, iters, 1, "v_cvt_pk_f16_f32");
   sweep<0, 6>(out, iters, 1, "v_max3_f32");
   sweep<0, 7>(out, iters, 1, "ds_read_b128");
@@ -139,7 +135,6 @@ int main(int argc, char** argv) {
   // two waves per SIMD: per-SIMD time per MFMA slot PAIR (both waves run the same loop); if wave B's VALU overlaps wave A's MFMA the
   // time stays at 2 x 34 cycles until the VALU of both waves fills the gaps
   sweep<0, 0, 512>(out, iters, 1, "two waves per SIMD, v_fma_f32");
-  sweep<0, 1, 512>(out, iters, 1, "two waves per SIMD, v_pk_fma_f32");
   sweep<0, 2, 512>(out, iters, 1, "two waves per SIMD, v_exp_f32");
   // gemm_as.h's operand forms: B operand from an AGPR, accumulators in VGPRs; the epilogue's reads of an idle accumulator block
   sweep<2, 0>(out, iters, 1, "B operand from AGPR + accumulators in VGPRs, v_fma_f32");

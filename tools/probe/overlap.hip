@@ -1,7 +1,7 @@
 // Issue-overlap probe for gfx950: how much VALU work hides behind v_mfma_f32_32x32x16_f16,
 //   (a) inside one wave (k independent fillers after every MFMA), and
 //   (b) across the two waves that share a SIMD (one MFMA-only, one VALU-only).
-// Build: hipcc --offload-arch=gfx950 -O2 overlap.hip -o overlap ; run on the GPU box.  Prints cycles per loop iteration
+// Build: hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops overlap.hip -o overlap ; run on an MI355X.  Prints cycles per loop iteration
 // (s_memtime, 100 MHz-independent: wall clock of the shader clock domain) for one wave per SIMD unless stated.
 #include <hip/hip_runtime.h>
 #include <cstdio>

@@ -1,6 +1,6 @@
 // Issue-overlap probe 2 (round 3) for gfx950, one wave per SIMD: what an LDS fragment read, a transpose read and a mixed
 // softmax filler set cost beside v_mfma_f32_32x32x16_f16, with the MFMA accumulators in architectural VGPRs or in AGPRs and the
-// A operand in a VGPR or an AGPR.  Build: hipcc --offload-arch=gfx950 -O2 overlap2.hip -o overlap2.  Prints shader cycles per
+// A operand in a VGPR or an AGPR.  Build: hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops overlap2.hip -o overlap2.  Prints shader cycles per
 // loop iteration (4 MFMAs = 128 matrix-pipe cycles).
 #include <hip/hip_runtime.h>
 #include <cstdio>

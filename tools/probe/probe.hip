@@ -2,7 +2,7 @@
 // Verifies (on a real MI355X) the lane layouts the kernels and the host
 // emulator (tools/hostemu) assume: MFMA 32x32x16 / 16x16x32 (f16, bf16),
 // global_load_lds 16B, ds_read_b64_tr_b16, v_permlane32_swap, f64 atomics.
-// Build: hipcc --offload-arch=gfx950 -O2 probe.hip -o probe ; run on GPU.
+// Build: hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops probe.hip -o probe ; run on GPU.
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>
