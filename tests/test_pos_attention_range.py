@@ -262,3 +262,19 @@ def test_some_biases_at_the_end_of_the_range(backend, dtype, which, request):
         within(t, want[n], want["tol_" + n], n)
     if which != "lowest":
         assert bool((lse == MOST).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("H,KH", [(1, 1), (4, 2)])
+def test_large_scores_in_some_rows_only(backend, dtype, H, KH, with_bias, request):
+    """waves with large scores beside waves without, in one workgroup, and rows of both kinds in one tile of the dK / dV pass (the bounds of the other
+    rows' gradients stay narrow)"""
+    N = 330
+    q = randn(1, 1, N, H * 64)
+    for a, b in ((32, 40), (100, 101), (160, 192), (300, 330)):
+        q[:, a:b] *= 4000
+    k, v, do = randn(2, 1, N, KH * 64), randn(3, 1, N, KH * 64), 0.1 * randn(4, 1, N, H * 64)
+    q, k, v, do = (t.to(dtype) for t in (q, k, v, do))
+    for window, sinks in (((-1, -1), 0), ((60, 0), 5)):
+        check_backward(ctx_of(backend, dtype, request), q, k, v, do, H, KH, window=window, sinks=sinks, bias=bias_of(with_bias, H, 9))
