@@ -84,8 +84,8 @@ STAR_DEV float gelu_erf(float x) {
   return fmaxf(x, 0.f) - ax * fast_exp2(p);
 }
 
-// the same on a PAIR of values: the degree-7 polynomial as seven v_pk_fma_f32 (packed fp32 is full rate on CDNA3/4: half the
-// instructions of two scalar chains; each element sees the same fma sequence as in gelu_erf -- bit-identical).  The GEGLU epilogues
+// the same on a PAIR of values, two independent chains of seven fma side by side (scalar instructions: the library is built without packed fp32);
+// each element sees the same fma sequence as in gelu_erf -- bit-identical.  The GEGLU epilogues
 // are VALU-bound (the A-stationary kernel's exceeds what 80 MFMAs shadow; the persistent tile's runs with the matrix pipe idle).
 using f32x2 = vec<float, 2>;
 STAR_DEV f32x2 gelu_erf2(f32x2 x) {

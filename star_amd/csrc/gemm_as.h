@@ -56,10 +56,10 @@ gemm_astat_kernel(const GemmParams p) {
   char* smem = dyn_smem();
   char* stg = smem + 2 * WTILE + wave_uniform((int)threadIdx.x >> 6) * STG;
   float* bias_lds = reinterpret_cast<float*>(smem + 2 * WTILE + 4 * STG);   // bias[N] | colsum[N]
-  // ILV >= 3: the GELU polynomial as scalar v_fma_f32 instead of v_pk_fma_f32.  Measured (tools/probe/mfma_valu_overlap.hip,
-  // profiles/r04_probe_mfma_valu_overlap.txt): a wave's v_fma_f32 ride in the shadow of its own MFMAs (4 per MFMA for free, 4.3
-  // cycles each beyond), its v_pk_fma_f32 do NOT (MFMA + 16 + 4.4 cycles each, no overlap at all) -- packed fp32 only pays where no
-  // MFMA is in flight.  ILV 3 = 1 + scalar, 4 = 0 + scalar, 5 = 2 + scalar.
+  // ILV >= 3: the GELU polynomial one value after the other instead of in pairs (gelu_erf2): 3 = 1, 4 = 0, 5 = 2 with it.  Both are scalar v_fma_f32 --
+  // the library is built without packed fp32 -- and differ in the order of the chains and in the group sizes below.  Measured
+  // (tools/probe/mfma_valu_overlap.hip, profiles/r04_probe_mfma_valu_overlap.txt): a wave's v_fma_f32 ride in the shadow of its own MFMAs
+  // (4 per MFMA for free, 4.3 cycles each beyond).
   // ILV 6: the product placement with the units re-ordered so that the two row blocks of a column quad are CONSECUTIVE and share one
   // fetch of its column sums / biases: 16 instead of 32 ds_read_b128 per tile and wave.  (Per W tile a CU's LDS moves 160 KB of W
   // fragments + 128 KB of these broadcast reads + 40 KB of staging and flush + the 40 KB DMA fill: ~2100 LDS-array cycles against 2560
@@ -275,7 +275,7 @@ gemm_astat_kernel(const GemmParams p) {
       }
       // ILV 1: this step's 4 MFMAs, each followed by a quarter of its VALU.  ILV 2 (GEGLU): whole units as in ILV 0, but the fence
       // between the unit's step and the next one is dropped and the pair's 8 MFMAs are each followed by an eighth of the unit
-      // (two independent polynomial chains side by side: no s_nop between dependent v_pk_fma_f32)
+      // (two independent polynomial chains side by side)
       constexpr bool PAIR = ILVP == 2 && GEGLU != 0;
       if constexpr (DRAIN && ILVP != 0 && !PAIR && ks < (GEGLU ? 2 * NU : NU)) {
         constexpr int VPER = GEGLU ? (SCALAR ? 12 : 10) : (ILVP == 2 ? 4 : 6);

@@ -13,14 +13,19 @@ constexpr int PA_NOLIM = 1 << 30;
 
 static bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-constexpr int PA_COMP_SPAN = 512;         // rows that see at most this many keys: P and dS with what their rounding left (COMP)
+// Rows that see at most this many keys: P and dS with what their rounding left (COMP), so that an output is off by its own rounding alone; above,
+// by 1.38 - 1.46 times that at every length.  What it costs, f16, 16 heads, all keys visible, us without / with: 16 x 128 tokens forward 15.2 / 15.1,
+// backward 34.6 / 33.0; 16 x 226 16.1 / 16.8, 46 / 54; 8 x 512 19.3 / 22.8, 69 / 85; 8 x 768 32.6 / 48, 142 / 179; 4 x 1024 30 / 37, 113 / 140;
+// 1 x 4096 94 / 124, 378 / 488: a few us while a call is mostly latency, a quarter to a half of the call from there on
+constexpr int PA_COMP_SPAN = 512;
 
 struct PPlan { int gp, rows, units, qb, nw, nq, nblk, nsplit, per, comp; };
 // the dK / dV pass: units (sequence, K / V head), key blocks, how many of them hold first tokens, in how many parts each kind, slots per unit
 struct PKPlan { int units, nblk, sblk, split_s, split_n, slots; size_t part_slots; };
 
 // Which form, and how many splits of the key tiles.  Up to 32 rows (a token's heads of one group, a few tokens): one wave per workgroup, and
-// as many workgroups as five per compute unit (LDS holds five), at least four tiles each.  More rows: 256-row workgroups where they give every
+// about ten workgroups per compute unit, at least four tiles each (LDS holds five at a time; with a bias's table four, from a reach of 900 three, which
+// the count does not ask for).  More rows: 256-row workgroups where they give every
 // compute unit its two, else 128-row ones, split along the keys while fewer than half of the places are taken.
 static PPlan pa_plan(Ctx* ctx, const PAttnArgs& a, bool backward) {
   PPlan q{};
@@ -47,7 +52,7 @@ static PPlan pa_plan(Ctx* ctx, const PAttnArgs& a, bool backward) {
     if (tiles > all) tiles = all;
     const long long base = (long long)q.units * q.nblk, places = (q.nw == 1 ? 5 : 2) * cus;
     // tiles per split: the same for all, so that sequences of different lengths make different counts of equal shares; about two workgroups
-    // per place, which evens out what one to the place leaves (one frame of 1350 tokens against a cache: 117 -> 103 us; a token of 32 sequences: 65 -> 61 us)
+    // per place, which evens out what one to the place leaves (one frame of 1350 tokens against a cache: 117 -> 103 us; a token of 32 sequences: 65 -> 61 us in the kernels, 68 with the call)
     long long per = base > 0 ? (tiles * base + places - 1) / places : tiles;
     per = (per + 1) / 2;
     if (per < 4) per = 4;

@@ -8,8 +8,8 @@
 //
 // Layout as in attn5.h: S^T = K Q^T with the operands swapped, so that a lane owns one query row and its probabilities are the B operand
 // of O^T = V^T P^T in place; K / V tiles of 64 keys in LDS by DMA, two buffers.  What differs, and why:
-//   * Q is not scaled before the product (that would round it to 16 bits once more; with the rounding of P the outputs would be off by more
-//     than 1.5 x their own rounding): the scale, the bias and the running maximum meet in one fma per score.
+//   * Q is not scaled before the product (that would round it to 16 bits once more, beside P): the scale, the bias and the running maximum meet
+//     in one fma per score.
 //   * A tile is "plain" when every row of the workgroup sees all of its keys and the bias is one constant there (past +-R it is: the far
 //     tiles, nearly all of a long sequence).  Plain tiles take the lazy path: P = exp2(fma(s, c, off)) against the running maximum as it
 //     stands, the row sum as overflow probe.  Every other tile, every tile until each row of the wave has seen one, and every tile of a wave
@@ -23,15 +23,16 @@
 //   * Few rows against long key ranges (a decoding step): the key tiles are dealt to NSPLIT workgroups in equal shares -- sequences of
 //     different lengths make different counts of shares -- each writes its (m, l, O) of the rows in fp32, pattn_combine_kernel joins them
 //     in a fixed order.
-// What bounds it, measured: long inputs the softmax's vector work beside the matrix unit (f16, 17 776 tokens, 16 heads, a window of 5400 either
-// way: 775 - 825 us, 0.85 PFLOP/s of the visible pairs; 32 rows per wave instead of 64 would read each fragment twice); a chunk of 1350 tokens against
-// a window of 10 800, 16 heads in groups of 4: 103 us, a twelfth of it the join.  A token at a time is bound by HBM: bf16, 32 sequences x 8 K / V
-// heads, 4160 of 32 800 keys: 58 us + 6 us of join, 4.6 TB/s of the 272 MB; 16 sequences x 16 heads of up to 8200 keys with a bias: 89 us + 6 us.  Few short rows
-// (8 x 226 tokens, 32 heads, a bias: 18 us) are the latency of one workgroup: table, four tiles, store.
+// What bounds it, measured: long inputs no one unit (f16, 17 776 tokens, 16 heads, a window of 5400 either way: 790 - 810 us, 0.85 PFLOP/s of the
+// visible pairs; vector unit busy 59 % of the cycles, matrix unit 41 %), and 1120 workgroups on the card's 512 places, the last round a fifth full
+// (32 rows per wave instead of 64 would read each fragment twice); a chunk of 1350 tokens against a window of 10 800, 16 heads in groups of 4: 104 us, 8 of
+// them the join, 1032 workgroups on 512 places.  A token at a time is bound by HBM: bf16, 32 sequences x 8 K / V heads, 4160 of 32 800 keys: 56 us + 5 us
+// of join, 4.8 TB/s of the 272 MB; 16 sequences x 16 heads of up to 8200 keys with a bias: 87 us + 6 us.  Few short rows (8 x 226 tokens, 32 heads, a
+// bias: 18 us) are latencies one after the other: lengths, Q, the table's two dependent loads, a barrier, then the first tile, four tiles, store.
 // NQ: 32-row blocks per wave (2: 256-row workgroups for long inputs, 1: 128 rows, more workgroups); NW = 1: a wave by itself, 32 rows.
 // COMP: P is rounded to the 16-bit type, and so is what the rounding left, and both take part in the second product: O is then off by its own
-// rounding alone.  Four more matrix instructions per 32 x 32 block, taken where they do not show: short rows (a few dozen roundings do not
-// average out there either) and the single-wave form, which waits for its keys.
+// rounding alone (1.00 x, without 1.28 - 1.41 x, the gradients 1.40 - 1.46 x).  Four more matrix instructions per 32 x 32 block, taken where they cost
+// little: rows that see few keys (PA_COMP_SPAN in pattn.cpp has both sides) and the single-wave form, which waits for its keys.
 #pragma once
 #include "attn.h"
 

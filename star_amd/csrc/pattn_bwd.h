@@ -20,13 +20,14 @@
 // COMP: as in the forward pass, dS and P with what their rounding left, for short rows.
 // Key blocks that many rows see (those of the first tokens: every row), or few blocks on many compute units, are dealt to several
 // workgroups along the rows; each writes its part in fp32, pattn_dkdv_join_kernel adds the parts in their order.
-// What bounds them: no one unit.  bf16, 2 x 4099 tokens, 16 heads, a bias: 1.0 ms (traced dQ 0.59, dK / dV 0.50 ms); 10 d flops a pair make
-// about 0.33 PFLOP/s, 0.6 with the products that are taken again (18 d).  Counters of the dQ kernel: vector unit busy 49 % of the cycles, matrix
-// unit 30 %, waves waiting 29 %, at 1.9 GHz.  Timed without its DMA, its exponentials or its last products (in copies, results wrong) each kernel
-// loses 6 - 10 %: what is left is the chain product -> exponential -> pack -> product of one tile, of two waves per SIMD.  Short sequences (4 x
-// 226 tokens, 16 heads: 35 + 21 + 5 us) are one such chain after the other and a launch each.  A window of 1024 over 4500 tokens, 16 heads in
-// groups of 4: 171 us (dQ 80, dK / dV 89, join 9 traced), 0.26 PFLOP/s.  Tried and no faster: 64 rows per wave in dQ (spills), three waves per
-// SIMD with a bias, halves of a tile in step with each other, the transposed fragments read before the exponentials.
+// What bounds them: no one unit, and how the workgroups fill the card.  bf16, 2 x 4099 tokens, 16 heads, a bias: 1.0 ms (traced dQ 0.53 - 0.56, dK / dV
+// 0.47 - 0.49 ms); 10 d flops a pair make 0.33 PFLOP/s, 0.6 with the products that are taken again (18 d).  Counters, dQ / dK dV: vector unit busy 56 /
+// 44 % of a busy compute unit's cycles, matrix unit 33 / 34 %, waves waiting 29 / 40 %; but a compute unit is busy 75 / 66 % of the time only: 1056 workgroups on
+// 512 places are two rounds and a few that make a third, and a block of three rows walks all its keys like a full one.  Short sequences (4 x 226 tokens, 16
+// heads: 30 + 22 + 5 us) are one chain of product -> exponential -> pack -> product after the other on 128 of 256 compute units, and a launch each.  A window of
+// 1024 over 4500 tokens, 16 heads in groups of 4: 173 us (dQ 80, dK / dV 86, join 10 traced), 0.26 PFLOP/s, compute units busy 70 / 74 %.  Tried and no faster:
+// 64 rows per wave in dQ (spills), three waves per SIMD with a bias, halves of a tile in step with each other, the transposed fragments read before the
+// exponentials.
 #pragma once
 #include "pattn.h"
 
