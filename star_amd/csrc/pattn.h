@@ -66,7 +66,9 @@ constexpr int PA_KT = 64, PA_TILE = PA_KT * 128;       // keys per tile, bytes o
 constexpr int PA_PART = 68;                            // floats per row of a split's partial result (16-byte rows)
 constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
 constexpr float PA_NINF = -__builtin_inff();
-constexpr float PA_LARGE = 4096.0f;                    // of scores in base 2: half a step of fp32 there is a relative 1.7e-4 of exp2
+// Of scores in base 2: half a step of fp32 there is a relative 1.7e-4 of exp2, a third of f16's half step; twice as much would no longer be small beside
+// it.  Logits of a trained layer are tens, and the rows above it take 1.1 - 1.6 x as long (video window 0.80 -> 1.18 ms, long bias backward 1.0 -> 1.6 ms)
+constexpr float PA_LARGE = 4096.0f;
 
 struct PRange { int n, qs; };                          // keys in hand, position of row 0 -- both clamped to what the kernels can index
 STAR_DEV PRange pa_range(const PAttnParams& p, int b) {
